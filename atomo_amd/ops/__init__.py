@@ -53,4 +53,4 @@ def ext():
     return _load(optional=False)
 
 
-from . import qsgd_ops, svd_ops, optim_ops  # noqa: E402,F401
+from . import qsgd_ops, svd_ops, optim_ops, logit_ops  # noqa: E402,F401

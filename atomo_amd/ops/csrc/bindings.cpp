@@ -11,6 +11,8 @@
 
 #include <cstdint>
 
+#include "op_bindings.h"
+
 extern "C" {
 void atomo_qsgd_pack_launch(const float*, float*, uint32_t*, int64_t, int, int,
                             bool, uint64_t, int, int, hipStream_t);
@@ -371,6 +373,7 @@ void sample_stage(torch::Tensor evecs, torch::Tensor evals,
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  register_logit_ops(m);
   m.def("sample_stage", &sample_stage,
         "fused on-device Bernoulli atom sampler + stage builder");
   m.def("jacobi_eigh", &jacobi_eigh, py::arg("grams"), py::arg("evals"),

@@ -1,0 +1,6 @@
+// The parts of the extension module that live in files of their own.
+#pragma once
+
+#include <torch/extension.h>
+
+void register_logit_ops(pybind11::module& m);

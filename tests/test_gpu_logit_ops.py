@@ -1,0 +1,376 @@
+"""label_logprobs and distill_loss on the GPU against the 64-bit oracle on the
+CPU, at the sizes and masks where the kernels can go wrong."""
+
+import math
+
+import pytest
+import torch
+
+from atomo_amd.ops import logit_ops
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24  # half a step of fp32, relative
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+SIZES = [(1, 1), (4, 3), (500, 10), (37, 100), (3, 511), (2, 1025), (5, 4099),
+         (2, 16385), (3, 50021), (1, 131072), (2, 70001)]
+
+
+def _steps(classes, spread):
+    """Roundings, in half steps, of a sum over the classes: a thread adds at
+    most classes / 64 terms one after the other, some 64 more join the
+    threads; exp(d) is off by its argument's rounding, 2 |d| half steps, and
+    exp itself by 4."""
+    return classes / 64 + 64 + 2 * spread + 4
+
+
+def _spread(z):
+    """The largest |d| that still counts: exp(-104) is 0 in fp32."""
+    wide = z.double()
+    finite = wide[torch.isfinite(wide)]
+    return float(min(104.0, (finite.max() - finite.min()))) if finite.numel() else 0.0
+
+
+def _logits(rows, classes, dtype, seed=0, mask=None, pad=0, offset=0):
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(rows, classes, generator=g) * 3
+    if mask == "some":
+        z[torch.rand(rows, classes, generator=g) < 0.3] = -math.inf
+    elif mask == "most":
+        z[torch.rand(rows, classes, generator=g) < 0.995] = -math.inf
+    elif mask == "lowest":
+        low = torch.rand(rows, classes, generator=g) < 0.3
+        z = z.to(dtype).masked_fill_(low, torch.finfo(dtype).min)
+    elif mask == "odd":
+        z[0] = -math.inf
+        z[-1, classes // 2] = math.nan
+        if rows > 2:
+            z[1, -1] = math.inf
+    elif mask == "ties":
+        z = torch.randint(-2, 2, (rows, classes), generator=g) * -0.0 + \
+            torch.randint(0, 2, (rows, classes), generator=g).float()
+    elif mask == "flat":
+        z[:] = 0.25
+    elif mask == "rising":
+        z = torch.linspace(-5, 5, classes).expand(rows, classes).contiguous()
+    z = z.to(dtype)
+    cuda = torch.zeros(rows, classes + pad + offset, dtype=dtype, device="cuda")
+    cuda = cuda[:, offset:offset + classes]
+    cuda.copy_(z)
+    return z, cuda
+
+
+def _same_odd(a, b):
+    """Equal where infinite or NaN; masks those out."""
+    assert torch.equal(a.isnan(), b.isnan())
+    assert torch.equal(a.isinf(), b.isinf())
+    assert torch.equal(a[a.isinf()], b[b.isinf()])
+    return torch.isfinite(a)
+
+
+def _check_logprobs(z, cuda, y, top):
+    want = logit_ops.label_logprobs(z, y, top=top)
+    got = logit_ops.label_logprobs(cuda, None if y is None else y.cuda(), top=top)
+    classes = z.shape[1]
+    u = U * _steps(classes, _spread(z))
+    for a, b in ((got.logprob, want.logprob), (got.top_logprob, want.top_logprob)):
+        if a is None:
+            continue
+        a, b = a.cpu().double(), b.double()
+        ok = _same_odd(a, b)
+        # log S: the sum's relative error; d: half a step of itself
+        assert ((a - b).abs()[ok] <= u + 4 * U * b.abs()[ok] + 4 * U * math.log(classes + 1)).all()
+    a, b = got.entropy.cpu().double(), want.entropy.double()
+    ok = _same_odd(a, b)
+    # T / S: two sums' errors on a quotient below the entropy
+    assert ((a - b).abs()[ok] <= 3 * u * (1 + b.abs()[ok]) + 4 * U * math.log(classes + 1)).all()
+    if top:
+        assert torch.equal(got.top_index.cpu(), want.top_index)
+
+
+def _labels(rows, classes, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    y = torch.randint(0, classes, (rows,), generator=g)
+    y[::3] = -100
+    return y
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,classes", SIZES)
+def test_logprobs_sizes(rows, classes, dtype):
+    z, cuda = _logits(rows, classes, dtype, seed=classes)
+    for top in sorted({0, 1, min(5, classes), min(128, classes)}):
+        _check_logprobs(z, cuda, _labels(rows, classes), top)
+
+
+@pytest.mark.parametrize("mask", ["some", "most", "lowest", "odd", "ties", "flat", "rising"])
+@pytest.mark.parametrize("rows,classes,dtype", [
+    (5, 10, F32), (4, 700, F16), (4, 5000, BF16), (3, 33333, F32), (600, 3000, BF16)])
+def test_logprobs_masks(rows, classes, dtype, mask):
+    z, cuda = _logits(rows, classes, dtype, seed=7, mask=mask)
+    _check_logprobs(z, cuda, _labels(rows, classes), min(20, classes))
+
+
+@pytest.mark.parametrize("pad,offset", [(1, 0), (0, 1), (5, 3), (64, 8)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logprobs_strides(dtype, pad, offset):
+    for rows, classes in ((9, 10), (6, 4097)):
+        z, cuda = _logits(rows, classes, dtype, pad=pad, offset=offset)
+        _check_logprobs(z, cuda, _labels(rows, classes), 7)
+    z, cuda = _logits(1, 300, dtype)
+    _check_logprobs(z.expand(5, 300), cuda.expand(5, 300), _labels(5, 300), 7)
+
+
+def test_logprobs_labels_outside_and_other_stream():
+    z, cuda = _logits(4, 50, F32)
+    y = torch.tensor([-100, 50, -1, 2 ** 40])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = logit_ops.label_logprobs(cuda, y.cuda(), top=3)
+    torch.cuda.current_stream().wait_stream(side)
+    assert out.logprob[0] == 0 and out.logprob[1:].isnan().all()
+    none = logit_ops.label_logprobs(cuda[:0], y[:0].cuda(), top=3)
+    assert none.top_index.shape == (0, 3)
+
+
+@pytest.mark.parametrize("rows,classes", [(1, 100000), (300, 10), (70, 5000)])
+def test_logprobs_in_a_graph(rows, classes):
+    _, first = _logits(rows, classes, BF16, seed=1)
+    y = _labels(rows, classes).cuda()
+    static = first.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        logit_ops.label_logprobs(static, y, top=4)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = logit_ops.label_logprobs(static, y, top=4)
+    for seed in range(4):
+        _, now = _logits(rows, classes, BF16, seed=seed)
+        static.copy_(now)
+        graph.replay()
+        want = logit_ops.label_logprobs(now, y, top=4)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+def _teacher(rows, classes, k, seed=5, repeat=False):
+    g = torch.Generator().manual_seed(seed)
+    if repeat:
+        index = torch.randint(0, classes, (rows, k), generator=g)
+    else:
+        index = torch.stack([torch.randperm(classes, generator=g)[:k] for _ in range(rows)])
+    return torch.randn(rows, k, generator=g) * 2, index
+
+
+def _terms(z, value, index, y, tau, weight):
+    """Sizes of the parts that the loss and the gradient are made of, in 64
+    bits: what roundings are relative to."""
+    d = z.double()
+    d = (d - d.amax(1, keepdim=True).clamp_min(-1e300)).nan_to_num(0, 0, -1e300)
+    p1 = torch.softmax(d, 1)
+    pt = torch.softmax(d / tau, 1)
+    there = value != -math.inf
+    t = value.double().masked_fill(~there, -1e300) / tau
+    share = torch.softmax(t, 1) * there
+    at = torch.where(there & (index >= 0) & (index < z.shape[1]), index, 0)
+    q = torch.zeros_like(p1).scatter_add_(1, at, share)
+    grad = weight * tau * (pt + q)
+    low = math.log(z.shape[1] + 1)
+    # roundings are relative to the distance itself, 3.4e38 for a class at the
+    # type's lowest value (half a step of that is 2e31); -inf stands at 1e300
+    # and only reaches losses that are infinite
+    dist = -(d / tau)
+    loss = weight * tau ** 2 * ((q * (dist + low)).sum(1) +
+                                (share * (t - t.amax(1, keepdim=True)).abs().clamp_max(1e30)).sum(1) + low)
+    if y is not None and weight < 1:
+        hot = torch.zeros_like(p1).scatter_(1, y.clamp(0, z.shape[1] - 1)[:, None], 1.0)
+        grad = grad + (1 - weight) * (p1 + hot)
+        loss = loss + (1 - weight) * ((hot * -d).sum(1) + low)
+    return loss, grad
+
+
+def _check_distill(z, cuda, value, index, y, tau, weight, reduction="mean", up=1.0):
+    rows, classes = z.shape
+    leaf = z.clone().requires_grad_()
+    kw = dict(temperature=tau, weight=weight, reduction=reduction)
+    want = logit_ops.distill_loss(leaf, value, index, y, **kw)
+    g = torch.Generator().manual_seed(11)
+    up = torch.rand(want.shape, generator=g) + 0.5 if reduction == "none" else torch.tensor(up)
+    # the oracle's gradient in 64 bits: of an fp32 leaf it rounds once more
+    (ref,) = torch.autograd.grad(want, leaf, up)
+    cl = cuda.detach().requires_grad_()
+    yc = None if y is None else y.cuda()
+    got = logit_ops.distill_loss(cl, value.cuda(), index.cuda(), yc, **kw)
+    (grad,) = torch.autograd.grad(got, cl, up.cuda(), retain_graph=True)
+    (again,) = torch.autograd.grad(got, cl, up.cuda())
+    # the second pass gives what the first gave
+    assert torch.equal(grad.isnan(), again.isnan())
+    assert torch.equal(grad.nan_to_num(), again.nan_to_num())
+    with torch.no_grad():
+        plain = logit_ops.distill_loss(cuda, value.cuda(), index.cuda(), yc, **kw)
+    assert torch.equal(plain.isnan(), got.isnan()) and torch.equal(plain.nan_to_num(), got.nan_to_num())
+    k = value.shape[1]
+    u = U * (_steps(classes, _spread(z) * max(1.0, 1 / tau)) + 2 * k + _spread(value))
+    loss_size, grad_size = _terms(z, value, index, y, tau, weight)
+    count = 1.0
+    counted = torch.ones(rows, dtype=torch.bool) if y is None else y != -100
+    if reduction == "mean":
+        count = max(1, int(counted.sum()))
+    a, b = got.cpu().double(), want.detach().double()
+    ok = _same_odd(a, b)
+    if reduction == "none":
+        tol = 2 * u * loss_size
+    else:
+        # the rows' errors, and those of adding them up
+        tol = (2 * u + U * (rows / 64 + 64)) * (loss_size * counted).sum() / count
+    assert ((a - b).abs() <= tol)[ok].all()
+    a, b = grad.cpu().double(), ref.double()
+    ok = _same_odd(a, b)
+    ups = up.double().abs()
+    ups = ups[:, None] if ups.dim() else ups
+    eps = torch.finfo(z.dtype).eps / 2
+    tiny = torch.finfo(z.dtype).smallest_normal * torch.finfo(z.dtype).eps
+    # the fp32 arithmetic, then one rounding on either side, then half a step
+    # next to zero on either side
+    tol = 2 * u * grad_size * ups / count + 2 * eps * b.abs() + 2 * tiny
+    assert ((a - b).abs() <= tol)[ok].all()
+    if y is not None:
+        assert (grad[(y == -100).cuda()] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,classes", SIZES)
+def test_distill_sizes(rows, classes, dtype):
+    z, cuda = _logits(rows, classes, dtype, seed=classes)
+    y = _labels(rows, classes)
+    if rows == 1:
+        y[0] = 0
+    for k in sorted({1, min(10, classes), min(128, classes)}):
+        value, index = _teacher(rows, classes, k)
+        _check_distill(z, cuda, value, index, y, 2.0, 0.7)
+        _check_distill(z, cuda, value, index, None, 1.0, 1.0, "sum")
+
+
+@pytest.mark.parametrize("tau,weight,reduction,up", [
+    (1.0, 0.5, "mean", 1.0), (4.0, 0.9, "none", 1.0), (0.25, 0.3, "sum", 3.0),
+    (2.0, 0.0, "mean", 0.0), (3.0, 1.0, "mean", -1.5), (2.0, 0.5, "mean", 1024.0)])
+@pytest.mark.parametrize("rows,classes,dtype", [(6, 100, F32), (5, 5003, BF16), (300, 1000, F16)])
+def test_distill_forms(rows, classes, dtype, tau, weight, reduction, up):
+    z, cuda = _logits(rows, classes, dtype)
+    value, index = _teacher(rows, classes, 17, repeat=True)
+    value[0, 3:] = -math.inf
+    index[0, 5] = classes + 4  # absent: never looked at
+    value[2] = -math.inf
+    y = _labels(rows, classes)
+    index[1, 0] = y[1]  # the label among the teacher's classes, twice
+    index[1, 9] = y[1]
+    _check_distill(z, cuda, value, index, y, tau, weight, reduction, up)
+
+
+@pytest.mark.parametrize("mask", ["some", "lowest", "odd", "flat"])
+@pytest.mark.parametrize("rows,classes,dtype", [(5, 10, F32), (4, 700, F16), (3, 33333, BF16)])
+def test_distill_masks(rows, classes, dtype, mask):
+    z, cuda = _logits(rows, classes, dtype, mask=mask)
+    value, index = _teacher(rows, classes, 6)
+    y = _labels(rows, classes)
+    y[1] = 1
+    for reduction in ("none", "mean"):
+        _check_distill(z, cuda, value, index, y, 2.0, 0.6, reduction)
+
+
+@pytest.mark.parametrize("classes", [50, 20000])
+def test_distill_wrong_entries(classes):
+    z, cuda = _logits(6, classes, F32)
+    value, index = _teacher(6, classes, 3)
+    index[0, 1], index[1, 2] = classes, -1
+    value[2, 0] = math.nan
+    y = torch.tensor([0, 0, 0, classes, -1, 2])
+    _check_distill(z, cuda, value, index, y, 2.0, 0.6, "none")
+
+
+@pytest.mark.parametrize("pad,offset", [(1, 0), (5, 3), (64, 8)])
+def test_distill_strides(pad, offset):
+    for dtype in (F32, F16):
+        z, cuda = _logits(6, 4097, dtype, pad=pad, offset=offset)
+        value, index = _teacher(6, 4097, 9)
+        _check_distill(z, cuda, value, index, None, 2.0, 1.0)
+
+
+def test_distill_all_rows_ignored():
+    _, cuda = _logits(3, 40, F32)
+    value, index = _teacher(3, 40, 4)
+    y = torch.full((3,), -100).cuda()
+    leaf = cuda.requires_grad_()
+    loss = logit_ops.distill_loss(leaf, value.cuda(), index.cuda(), y, weight=0.5)
+    loss.backward()
+    assert loss == 0 and (leaf.grad == 0).all()
+    none = logit_ops.distill_loss(cuda[:0], value[:0].cuda(), index[:0].cuda())
+    assert none == 0
+
+
+def test_distill_refuses_a_second_derivative_and_a_changed_input():
+    _, cuda = _logits(3, 40, F32)
+    value, index = (t.cuda() for t in _teacher(3, 40, 4))
+    leaf = cuda.requires_grad_()
+    loss = logit_ops.distill_loss(leaf, value, index)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, leaf, create_graph=True)
+    with pytest.raises(ValueError):
+        logit_ops.distill_loss(leaf, value.cpu(), index)
+    moved = leaf * 1.0
+    loss = logit_ops.distill_loss(moved, value, index)
+    with torch.no_grad():
+        moved.mul_(2.0)
+    with pytest.raises(RuntimeError):
+        (2.0 * loss).backward()
+
+
+@pytest.mark.parametrize("rows,classes,dtype", [(128, 100, F32), (3, 60000, BF16), (40, 5000, F16)])
+def test_distill_in_a_graph(rows, classes, dtype):
+    """Forward and backward captured, replayed between eager passes."""
+    _, first = _logits(rows, classes, dtype)
+    value, index = (t.cuda() for t in _teacher(rows, classes, 8))
+    y = _labels(rows, classes).cuda()
+    kw = dict(temperature=2.0, weight=0.5)
+    static = first.clone().requires_grad_()
+
+    def step(leaf):
+        loss = logit_ops.distill_loss(leaf, value, index, y, **kw)
+        (grad,) = torch.autograd.grad(loss, leaf)
+        return loss.detach(), grad
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = step(static)
+    for seed in range(4):
+        _, now = _logits(rows, classes, dtype, seed=seed)
+        with torch.no_grad():
+            static.copy_(now)
+        graph.replay()
+        want_loss, want = step(now.clone().requires_grad_())
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want_loss) and torch.equal(grad, want)
+
+
+def test_teacher_answers_feed_the_loss():
+    """The two together, as they are used: a teacher's alternatives, the
+    student's loss and gradient."""
+    rows, classes = 33, 12345
+    zt, teacher = _logits(rows, classes, BF16, seed=1)
+    zs, student = _logits(rows, classes, BF16, seed=2)
+    out = logit_ops.label_logprobs(teacher, top=64)
+    cpu = logit_ops.label_logprobs(zt, top=64)
+    assert torch.equal(out.top_index.cpu(), cpu.top_index)
+    _check_distill(zs, student, out.top_logprob.cpu(), out.top_index.cpu(),
+                   _labels(rows, classes), 2.0, 0.8)
