@@ -53,4 +53,6 @@ def ext():
     return _load(optional=False)
 
 
-from . import qsgd_ops, svd_ops, optim_ops, logit_ops  # noqa: E402,F401
+from . import (  # noqa: E402,F401
+    linear_ops, logit_ops, optim_ops, qsgd_ops, svd_ops,
+)

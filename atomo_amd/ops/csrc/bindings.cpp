@@ -373,6 +373,7 @@ void sample_stage(torch::Tensor evecs, torch::Tensor evals,
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  register_linear_ops(m);
   register_logit_ops(m);
   m.def("sample_stage", &sample_stage,
         "fused on-device Bernoulli atom sampler + stage builder");

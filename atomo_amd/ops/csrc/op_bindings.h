@@ -3,4 +3,5 @@
 
 #include <torch/extension.h>
 
+void register_linear_ops(pybind11::module& m);
 void register_logit_ops(pybind11::module& m);

@@ -1,0 +1,132 @@
+"""Fully connected layer with its epilogue in the product's kernel (kernels:
+ops/csrc/linear_kernels.hip).
+
+    y = act(x W^T + b) + residual        act: none, relu, gelu (erf), silu
+
+and its gradients.  ``models.fuse_linears`` puts it in the place of the model
+zoo's Linear (+ ReLU) layers (``--fused-linear``).  CUDA (= ROCm) tensors take
+the HIP kernels, CPU tensors the torch oracle (64-bit inside).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from . import ext
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _same(t: torch.Tensor, x: torch.Tensor, shape, name: str) -> torch.Tensor:
+    if t.dtype != x.dtype:
+        raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}")
+    if t.device != x.device:
+        raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
+    return t
+
+
+def _matrix(t: torch.Tensor) -> torch.Tensor:
+    """(..., columns) as (rows, columns) with contiguous rows."""
+    if t.dim() != 2:
+        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t
+
+
+def linear_act(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    activation: str = "none",
+    residual: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` for x (..., in), weight
+    (out, in), bias (out), residual (..., out), all of one type: fp32, bf16 or
+    fp16.
+
+    Products and sums are fp32 (fp32 operands are multiplied as such), the
+    result is rounded once.  Of gelu and silu the slope is kept for the
+    backward pass in the operands' type, and dy times the slope is rounded to
+    it before it is multiplied.  Rows may be strided; other layouts are copied
+    first.  The gradients cannot be differentiated again on a GPU.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(
+            f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"x must be fp32, bf16 or fp16, not {x.dtype}")
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError("weight must be (out, in), neither of them 0")
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"x must be (..., {k}), not {tuple(x.shape)}")
+    lead = x.shape[:-1]
+    _same(weight, x, (n, k), "weight")
+    if bias is not None:
+        _same(bias, x, (n,), "bias")
+    if residual is not None:
+        _same(residual, x, (*lead, n), "residual")
+    if x.is_cuda:
+        y = ext().linear_act(
+            _matrix(x), _matrix(weight),
+            None if bias is None else bias.contiguous(),
+            None if residual is None else _matrix(residual),
+            ACTIVATIONS[activation])
+        return y if len(lead) == 1 else y.view(*lead, n)
+    wide = None if bias is None else bias.double()
+    h = F.linear(x.double(), weight.double(), wide)
+    if activation == "relu":
+        h = h.relu()
+    elif activation != "none":
+        # 0 at -inf, their limit
+        h = h.clamp_min(-1e4)
+        h = F.gelu(h) if activation == "gelu" else F.silu(h)
+    if residual is not None:
+        h = h + residual.double()
+    return h.to(x.dtype)
+
+
+class FusedLinear(nn.Linear):
+    """``nn.Linear`` with its activation in the same kernel; same parameters,
+    same names."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True,
+                 activation: str = "none"):
+        super().__init__(in_features, out_features, bias)
+        if activation not in ACTIVATIONS:
+            raise ValueError(
+                f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
+        self.activation = activation
+
+    @classmethod
+    def of(cls, linear: nn.Linear, activation: str = "none") -> "FusedLinear":
+        """Takes over a layer's parameters (the same objects)."""
+        fused = cls.__new__(cls)
+        nn.Module.__init__(fused)
+        fused.in_features = linear.in_features
+        fused.out_features = linear.out_features
+        fused.weight, fused.bias = linear.weight, linear.bias
+        fused.activation = activation
+        return fused.train(linear.training)
+
+    def forward(self, x: torch.Tensor,
+                residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        weight, bias = self.weight, self.bias
+        if torch.is_autocast_enabled(x.device.type):
+            kind = torch.get_autocast_dtype(x.device.type)
+            x, weight = x.to(kind), weight.to(kind)
+            bias = bias if bias is None else bias.to(kind)
+            residual = residual if residual is None else residual.to(kind)
+        return linear_act(x, weight, bias, self.activation, residual)
+
+    def extra_repr(self) -> str:
+        return f"{super().extra_repr()}, activation={self.activation}"

@@ -23,6 +23,8 @@ ext = CUDAExtension(
         "atomo_amd/ops/csrc/atomo_kernels.hip",
         "atomo_amd/ops/csrc/svd_batched.hip",
         "atomo_amd/ops/csrc/jacobi_eigh.hip",
+        "atomo_amd/ops/csrc/linear_bindings.cpp",
+        "atomo_amd/ops/csrc/linear_kernels.hip",
         "atomo_amd/ops/csrc/logit_bindings.cpp",
         "atomo_amd/ops/csrc/logit_kernels.hip",
     ],
