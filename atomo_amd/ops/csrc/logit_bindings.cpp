@@ -8,7 +8,7 @@
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
-#include <limits>
+#include <algorithm>
 #include <tuple>
 
 #include "logit_kernels.h"
@@ -36,8 +36,7 @@ void check_logits(const Tensor& z) {
   TORCH_CHECK(z.dim() == 2 && z.size(1) >= 1, "logits must be (rows, classes)");
   TORCH_CHECK(z.size(1) == 1 || z.stride(1) == 1,
               "the classes of a row must be contiguous");
-  TORCH_CHECK(z.size(1) < std::numeric_limits<int32_t>::max(),
-              "too many classes");
+  TORCH_CHECK(z.size(1) <= (int64_t)1 << 30, "more than 2^30 classes");
   TORCH_CHECK(z.stride(0) >= 0, "logits must not have a negative stride");
 }
 
@@ -73,11 +72,28 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> label_logprobs(
   Tensor top_logprob = torch::empty({rows, top}, f32);
   Tensor top_index = torch::empty({rows, top}, f32.dtype(torch::kInt64));
   if (rows > 0) {
-    atomo_label_logprobs_launch(
-        z.data_ptr(), type_of(z), z.stride(0), rows, (int)classes, y, ignore,
-        (int)top, y ? logprob.data_ptr<float>() : nullptr,
-        entropy.data_ptr<float>(), top_logprob.data_ptr<float>(),
-        top_index.data_ptr<int64_t>(), cur_stream());
+    AtomoLogprobs a{};
+    a.logits = z.data_ptr();
+    a.labels = y;
+    a.logprob = y ? logprob.data_ptr<float>() : nullptr;
+    a.entropy = entropy.data_ptr<float>();
+    a.top_logprob = top_logprob.data_ptr<float>();
+    a.top_index = top_index.data_ptr<int64_t>();
+    a.row_stride = z.stride(0);
+    a.rows = rows;
+    a.ignore = ignore;
+    a.type = type_of(z);
+    a.classes = (int)classes;
+    a.top = (int)top;
+    a.splits = atomo_logit_splits(rows, a.classes, a.type, &a.part_size);
+    Tensor part_stat, part_keys;
+    if (a.splits > 1) {
+      part_stat = torch::empty({rows, a.splits, 3}, f32);
+      part_keys = torch::empty({rows, a.splits, top}, top_index.options());
+      a.part_stat = part_stat.data_ptr<float>();
+      a.part_keys = part_keys.data_ptr<int64_t>();
+    }
+    atomo_label_logprobs_launch(&a, cur_stream());
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
   return {logprob, entropy, top_logprob, top_index};
@@ -86,10 +102,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> label_logprobs(
 enum Reduction { kNone = 0, kMean = 1, kSum = 2 };
 
 struct DistillLoss : public torch::autograd::Function<DistillLoss> {
+  // `wanted`: a gradient may be asked for
   static Tensor forward(AutogradContext* ctx, const Tensor& z,
                         const Tensor& values, const Tensor& index,
                         const c10::optional<Tensor>& labels_opt, double tau,
-                        double weight, int64_t ignore, int64_t reduction) {
+                        double weight, int64_t ignore, int64_t reduction,
+                        bool wanted) {
     const Tensor labels = labels_opt.value_or(Tensor());
     check_logits(z);
     check_rows(values, z, torch::kFloat32, "teacher_value");
@@ -99,85 +117,159 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
                 "teacher_value and teacher_index must be (rows, k) with k <= ",
                 ATOMO_LOGIT_TOP_MAX);
     const c10::DeviceGuard guard(z.device());
-    const int64_t* y = labels_of(labels, z);
-    const int64_t rows = z.size(0);
-    // without the teacher's weight its entries are not looked at
-    const int k = weight == 0.0 ? 0 : (int)values.size(1);
-    const auto f32 = z.options().dtype(torch::kFloat32);
-    Tensor row_loss = torch::empty({rows}, f32);
-    Tensor stats = torch::empty({rows, 3}, f32);
-    Tensor inverse;  // one over the counted rows, where labels decide them
-    double factor = 1.0;
-    if (reduction == kMean) {
-      if (y)
-        inverse = torch::empty({1}, f32);
-      else
-        factor = 1.0 / (double)std::max<int64_t>(rows, 1);
-    }
-    Tensor loss = reduction == kNone ? row_loss : torch::empty({}, f32);
     const hipStream_t stream = cur_stream();
-    float* inv = inverse.defined() ? inverse.data_ptr<float>() : nullptr;
-    if (inv) {
-      atomo_distill_count_launch(y, rows, ignore, inv, stream);
-      C10_HIP_KERNEL_LAUNCH_CHECK();
+    const int64_t rows = z.size(0);
+    const auto f32 = z.options().dtype(torch::kFloat32);
+
+    AtomoDistill a{};
+    a.labels = labels_of(labels, z);
+    a.weight = (float)weight;
+    // without the teacher's weight its entries are not looked at
+    a.k = weight == 0.0 ? 0 : (int)values.size(1);
+    a.tau = weight == 0.0 ? 1.f : (float)tau;
+    a.inv_tau = 1.f / a.tau;
+    a.ignore = ignore;
+    a.factor = 1.f;
+    if (a.labels == nullptr || weight == 1.0)
+      a.mode = ATOMO_DISTILL_SOFT;
+    else if (a.tau == 1.f)
+      a.mode = ATOMO_DISTILL_TAU1;
+    else if (a.tau == 2.f)
+      a.mode = ATOMO_DISTILL_TAU2;
+    else if (a.tau == 4.f)
+      a.mode = ATOMO_DISTILL_TAU4;
+    else
+      a.mode = ATOMO_DISTILL_ANY;
+    Tensor inverse;  // one over the counted rows
+    if (reduction == kMean && a.labels) {
+      a.count = rows <= ATOMO_LOGIT_COUNT_ROWS;
+      if (!a.count) {
+        inverse = torch::empty({1}, f32);
+        atomo_distill_count_launch(a.labels, rows, ignore,
+                                   inverse.data_ptr<float>(), stream);
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+      }
+    } else if (reduction == kMean) {
+      a.factor = 1.f / (float)std::max<int64_t>(rows, 1);
+    }
+    describe(a, z, values, index, inverse);
+
+    const bool fits = atomo_distill_fits(rows, a.classes, a.type);
+    // The gradient of a mean or a sum is written along with the loss, for an
+    // upstream gradient of 1; the backward pass writes it anew where that is
+    // not so.  Not in fp16: a scaled loss is the rule there, as its smallest
+    // steps lose most of an unscaled gradient.
+    const bool fused = wanted && fits && reduction != kNone &&
+                       z.scalar_type() != torch::kFloat16;
+    // one read of a short row by one wave; long ones are swept
+    const bool in_registers = fused || atomo_distill_short(a.classes, a.type);
+    if (in_registers) {
+      a.splits = 1;
+    } else {
+      a.splits = atomo_logit_splits(rows, a.classes, a.type, &a.part_size);
+    }
+    Tensor row_loss = torch::empty({rows}, f32);
+    Tensor stats = torch::empty({rows, a.splits, 3}, f32);
+    Tensor loss = reduction == kNone ? row_loss : torch::empty({}, f32);
+    Tensor grad;
+    a.row_loss = row_loss.data_ptr<float>();
+    a.stats = stats.data_ptr<float>();
+    if (fused) {
+      grad = torch::empty({rows, z.size(1)}, z.options());
+      a.grad = grad.data_ptr();
     }
     if (rows > 0) {
-      atomo_distill_loss_launch(
-          z.data_ptr(), type_of(z), z.stride(0), rows, (int)z.size(1),
-          values.data_ptr<float>(), index.data_ptr<int64_t>(), k, y, ignore,
-          (float)tau, (float)weight, row_loss.data_ptr<float>(),
-          stats.data_ptr<float>(), stream);
+      if (in_registers)
+        atomo_distill_fused_launch(&a, stream);
+      else
+        atomo_distill_loss_launch(&a, stream);
       C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     if (reduction != kNone) {
-      atomo_distill_sum_launch(row_loss.data_ptr<float>(), rows, inv,
-                               (float)factor, loss.data_ptr<float>(), stream);
+      atomo_distill_sum_launch(&a, loss.data_ptr<float>(), stream);
       C10_HIP_KERNEL_LAUNCH_CHECK();
     }
-    ctx->save_for_backward({z, values, index, labels, stats, inverse});
-    ctx->saved_data["tau"] = tau;
-    ctx->saved_data["weight"] = weight;
-    ctx->saved_data["ignore"] = ignore;
-    ctx->saved_data["k"] = (int64_t)k;
-    ctx->saved_data["factor"] = factor;
-    ctx->saved_data["per_row"] = reduction == kNone;
+    if (wanted) {
+      ctx->save_for_backward({z, values, index, labels, stats, inverse});
+      auto& d = ctx->saved_data;
+      d["tau"] = (double)a.tau;
+      d["weight"] = weight;
+      d["ignore"] = ignore;
+      d["factor"] = (double)a.factor;
+      d["k"] = (int64_t)a.k;
+      d["mode"] = (int64_t)a.mode;
+      d["splits"] = (int64_t)a.splits;
+      d["count"] = a.count != 0;
+      d["per_row"] = reduction == kNone;
+      if (fused) d["grad"] = grad;
+    }
     return loss;
+  }
+
+  static void describe(AtomoDistill& a, const Tensor& z, const Tensor& values,
+                       const Tensor& index, const Tensor& inverse) {
+    a.logits = z.data_ptr();
+    a.values = values.data_ptr<float>();
+    a.index = index.data_ptr<int64_t>();
+    a.inverse = inverse.defined() ? inverse.data_ptr<float>() : nullptr;
+    a.row_stride = z.stride(0);
+    a.rows = z.size(0);
+    a.type = type_of(z);
+    a.classes = (int)z.size(1);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list up_list) {
     TORCH_CHECK(!c10::GradMode::is_enabled(),
                 "distill_loss has no second derivative (create_graph)");
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &z = saved[0], &labels = saved[3], &inverse = saved[5];
+    const Tensor &z = saved[0], &labels = saved[3], &stats = saved[4];
     const c10::DeviceGuard guard(z.device());
-    const int64_t rows = z.size(0);
-    const bool per_row = ctx->saved_data["per_row"].toBool();
+    auto& d = ctx->saved_data;
     const Tensor up = up_list[0].to(torch::kFloat32).contiguous();
-    Tensor grad = torch::empty({rows, z.size(1)}, z.options());
-    if (rows > 0) {
-      atomo_distill_grad_launch(
-          z.data_ptr(), type_of(z), z.stride(0), rows, (int)z.size(1),
-          saved[1].data_ptr<float>(), saved[2].data_ptr<int64_t>(),
-          (int)ctx->saved_data["k"].toInt(), labels_of(labels, z),
-          ctx->saved_data["ignore"].toInt(),
-          (float)ctx->saved_data["tau"].toDouble(),
-          (float)ctx->saved_data["weight"].toDouble(),
-          saved[4].data_ptr<float>(), up.data_ptr<float>(), per_row,
-          inverse.defined() ? inverse.data_ptr<float>() : nullptr,
-          (float)ctx->saved_data["factor"].toDouble(), grad.data_ptr(),
-          cur_stream());
+    AtomoDistill a{};
+    a.labels = labels_of(labels, z);
+    a.weight = (float)d["weight"].toDouble();
+    a.k = (int)d["k"].toInt();
+    a.tau = (float)d["tau"].toDouble();
+    a.inv_tau = 1.f / a.tau;
+    a.ignore = d["ignore"].toInt();
+    a.factor = (float)d["factor"].toDouble();
+    a.mode = (int)d["mode"].toInt();
+    a.splits = (int)d["splits"].toInt();
+    a.count = d["count"].toBool();
+    describe(a, z, saved[1], saved[2], saved[5]);
+    a.stats = stats.data_ptr<float>();
+    a.up = up.data_ptr<float>();
+    a.up_per_row = d["per_row"].toBool();
+    // The gradient that the forward pass wrote is given away once; a further
+    // backward pass makes its own.
+    Tensor grad;
+    const auto found = d.find("grad");
+    if (found != d.end()) {
+      grad = found->second.toTensor();
+      d.erase(found);
+      a.skip_one = 1;
+    } else {
+      grad = torch::empty({z.size(0), z.size(1)}, z.options());
+    }
+    a.grad = grad.data_ptr();
+    a.grad_splits =
+        atomo_logit_splits(z.size(0), a.classes, a.type, &a.grad_part);
+    if (z.size(0) > 0) {
+      atomo_distill_grad_launch(&a, cur_stream());
       C10_HIP_KERNEL_LAUNCH_CHECK();
     }
-    return {grad, Tensor(), Tensor(), Tensor(), Tensor(),
-            Tensor(), Tensor(), Tensor()};
+    return {grad,     Tensor(), Tensor(), Tensor(), Tensor(),
+            Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
 Tensor distill_loss(const Tensor& z, const Tensor& values, const Tensor& index,
                     const c10::optional<Tensor>& labels, double tau,
                     double weight, int64_t ignore, int64_t reduction) {
+  const bool wanted = c10::GradMode::is_enabled() && z.requires_grad();
   return DistillLoss::apply(z, values, index, labels, tau, weight, ignore,
-                            reduction);
+                            reduction, wanted);
 }
 
 }  // namespace

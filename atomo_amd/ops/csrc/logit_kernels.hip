@@ -19,8 +19,6 @@
 // log probabilities are -inf, its entropy 0, its loss and gradient 0.  A row
 // with NaN or +inf gives NaN.
 
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -33,77 +31,158 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_huge_valf();
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / WAVE;
-constexpr int kTopMax = ATOMO_LOGIT_TOP_MAX;
 
-__device__ __forceinline__ float widen(float x) { return x; }
-__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
-__device__ __forceinline__ float widen(__hip_bfloat16 x) {
-  return __bfloat162float(x);
-}
-template <typename T>
-__device__ __forceinline__ T narrow(float x);
-template <>
-__device__ __forceinline__ float narrow<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half narrow<__half>(float x) {
-  return __float2half(x);
-}
-template <>
-__device__ __forceinline__ __hip_bfloat16 narrow<__hip_bfloat16>(float x) {
-  return __float2bfloat16(x);
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// rows may start at any element: vectors in memory are aligned to elements
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+
+__device__ __forceinline__ float nan_value() { return __builtin_nanf(""); }
+
+// -- element types: kVec elements in 16 bytes ---------------------------------
+struct F32 {
+  using Raw = uint32_t;
+  static constexpr int kVec = 4;
+  static constexpr Raw kLowest = 0xFF800000u;  // -inf
+  using Mem = u32x4_a4;
+  __device__ static float widen(Raw r) { return __uint_as_float(r); }
+  __device__ static Raw narrow(float f) { return __float_as_uint(f); }
+};
+struct BF16 {
+  using Raw = uint16_t;
+  static constexpr int kVec = 8;
+  static constexpr Raw kLowest = 0xFF80u;
+  using Mem = u32x4_a2;
+  __device__ static float widen(Raw r) {
+    return __uint_as_float((uint32_t)r << 16);
+  }
+  __device__ static Raw narrow(float f) {
+    return __builtin_bit_cast(Raw, (__bf16)f);
+  }
+};
+struct F16 {
+  using Raw = uint16_t;
+  static constexpr int kVec = 8;
+  static constexpr Raw kLowest = 0xFC00u;
+  using Mem = u32x4_a2;
+  __device__ static float widen(Raw r) {
+    return (float)__builtin_bit_cast(_Float16, r);
+  }
+  __device__ static Raw narrow(float f) {
+    return __builtin_bit_cast(Raw, (_Float16)f);
+  }
+};
+
+template <typename E>
+__device__ __forceinline__ float element(const u32x4& v, int e) {
+  if constexpr (E::kVec == 4)
+    return E::widen(v[e]);
+  else
+    return E::widen((uint16_t)(v[e / 2] >> (e % 2 * 16)));
 }
 
+// 16 bytes from element `at` on; from `end` on, -inf
+template <typename E>
+__device__ __forceinline__ u32x4 load_vec(const typename E::Raw* z, int at,
+                                          int end) {
+  if (at + E::kVec <= end) return *(const typename E::Mem*)(z + at);
+  u32x4 v;
+  if (at >= end) {
+    constexpr uint32_t two = E::kLowest | (uint32_t)E::kLowest << 16;
+    constexpr uint32_t low = E::kVec == 4 ? (uint32_t)E::kLowest : two;
+    return u32x4{low, low, low, low};
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (E::kVec == 4) {
+      v[i] = at + i < end ? z[at + i] : E::kLowest;
+    } else {
+      const uint32_t lo = at + 2 * i < end ? z[at + 2 * i] : E::kLowest;
+      const uint32_t hi = at + 2 * i + 1 < end ? z[at + 2 * i + 1] : E::kLowest;
+      v[i] = lo | hi << 16;
+    }
+  }
+  return v;
+}
+
+template <typename E>
+__device__ __forceinline__ void store_vec(typename E::Raw* g, int at, int end,
+                                          const float* x) {
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (E::kVec == 4)
+      v[i] = E::narrow(x[i]);
+    else
+      v[i] = (uint32_t)E::narrow(x[2 * i]) |
+             (uint32_t)E::narrow(x[2 * i + 1]) << 16;
+  }
+  if (at + E::kVec <= end) {
+    *(typename E::Mem*)(g + at) = v;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < E::kVec; ++e)
+    if (at + e < end) g[at + e] = E::narrow(x[e]);
+}
+
+// -- sums ---------------------------------------------------------------------
 // e^d for d <= 0 (or NaN); e^-inf = 0
 __device__ __forceinline__ float exp_of(float d) {
   return __builtin_amdgcn_exp2f(d * kLog2e);
 }
 
-// Order of the classes by logit: whole numbers that rise with the value, NaN
-// above all, -0 equal to +0; the lowest class first among equals.  No class
-// has key 0.
-__device__ __forceinline__ uint32_t order_of(float x) {
-  if (x != x) return 0xFFFFFFFFu;
-  const uint32_t b = __float_as_uint(x + 0.0f);
-  return (b >> 31) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t column) {
-  return ((uint64_t)order_of(x) << 32) | (0xFFFFFFFFu - column);
-}
-__device__ __forceinline__ uint32_t column_of(uint64_t key) {
-  return 0xFFFFFFFFu - (uint32_t)key;
-}
-
-// Maximum and the sums relative to it; joined pairwise in a fixed order.
-struct Stat {
-  float m, s, t;
-};
-
 // 0 stands in for a maximum of -inf: exp(-inf - 0) is 0, not NaN
 __device__ __forceinline__ float origin(float m) { return m == -kInf ? 0.f : m; }
 
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-  Stat r;
-  r.m = fmaxf(a.m, b.m);
-  const float o = origin(r.m);
-  // the floor keeps 0 * -inf out of t
-  const float da = fmaxf(a.m - o, -1e30f), db = fmaxf(b.m - o, -1e30f);
-  const float fa = exp_of(da), fb = exp_of(db);
-  r.s = a.s * fa + b.s * fb;
-  r.t = (a.t + da * a.s) * fa + (b.t + db * b.s) * fb;
-  return r;
+// the exponent that brings a sum relative to `from` to one relative to `to`;
+// its floor keeps 0 * -inf out of what it is multiplied with
+__device__ __forceinline__ float shift(float from, float to) {
+  return fmaxf(from - origin(to), -1e30f);
 }
 
-__device__ __forceinline__ Stat wave_join(Stat v) {
+// m, S and T of a part of a row
+struct Stat {
+  float m, s, t;
+  __device__ static Stat none() { return {-kInf, 0.f, 0.f}; }
+  __device__ void move(float to) {
+    const float d = shift(m, to), f = exp_of(d);
+    t = (t + d * s) * f;
+    s *= f;
+    m = to;
+  }
+};
+// m, S and S_t
+struct Sums {
+  float m, s, t;
+  __device__ static Sums none() { return {-kInf, 0.f, 0.f}; }
+  __device__ void move(float to, float inv_tau) {
+    const float d = shift(m, to);
+    s *= exp_of(d);
+    t *= exp_of(d * inv_tau);
+    m = to;
+  }
+};
+template <typename P, typename... A>
+__device__ __forceinline__ P join(P a, P b, A... tau) {
+  const float m = fmaxf(a.m, b.m);
+  a.move(m, tau...);
+  b.move(m, tau...);
+  a.s += b.s;
+  a.t += b.t;
+  return a;
+}
+
+// all lanes get the sum; a fixed order of additions
+template <typename P, typename... A>
+__device__ __forceinline__ P wave_join(P v, A... tau) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
-    Stat o;
+    P o;
     o.m = __shfl_xor(v.m, off, WAVE);
     o.s = __shfl_xor(v.s, off, WAVE);
     o.t = __shfl_xor(v.t, off, WAVE);
-    // the same operand order in both lanes of a pair: one result for all
-    v = (threadIdx.x & off) ? join(o, v) : join(v, o);
+    v = (threadIdx.x & off) ? join(o, v, tau...) : join(v, o, tau...);
   }
   return v;
 }
@@ -118,121 +197,841 @@ __device__ __forceinline__ float wave_sum(float v) {
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, WAVE);
   return v;
 }
-__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
+
+// joins the waves' parts; `lds` holds one for each wave
+template <int kThreads, typename P, typename... A>
+__device__ __forceinline__ P block_join(P v, P* lds, A... tau) {
+  v = wave_join(v, tau...);
+  if constexpr (kThreads > WAVE) {
+    if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = v;
+    __syncthreads();
+    v = lds[0];
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const uint64_t o = __shfl_xor((unsigned long long)v, off, WAVE);
-    v = o > v ? o : v;
+    for (int w = 1; w < kThreads / WAVE; ++w) v = join(v, lds[w], tau...);
   }
   return v;
 }
 
-__device__ __forceinline__ float block_max(float v, float* lds) {
-  v = wave_max(v);
-  __syncthreads();
-  if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = v;
-  __syncthreads();
-  float r = lds[0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) r = fmaxf(r, lds[i]);
-  return r;
-}
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-  v = wave_sum(v);
-  __syncthreads();
-  if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = v;
-  __syncthreads();
-  float r = lds[0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) r += lds[i];
-  return r;
-}
-
-// log softmax of one logit; `o` = origin(m)
+// log softmax of one logit
 __device__ __forceinline__ float log_prob(float z, float m, float log_s) {
   if (m == -kInf && log_s == -kInf) return -kInf;  // an empty row
   return (z - origin(m)) - log_s;
 }
 
-// ---------------------------------------------------------------------------
-// log probability, entropy, top alternatives: one workgroup a row
-// ---------------------------------------------------------------------------
-template <typename T>
+// Rows are spread over two dimensions of the grid: one dimension holds fewer
+// than 2^32 threads.
+constexpr int kGridRows = 1 << 18;
+__device__ __forceinline__ int64_t grid_row(int splits) {
+  return (int64_t)blockIdx.y * kGridRows + blockIdx.x / splits;
+}
+dim3 grid_of(int64_t rows, int splits) {
+  const int64_t x = rows < kGridRows ? rows : kGridRows;
+  return dim3((unsigned)(x * splits), (unsigned)((rows + x - 1) / x));
+}
+
+// -- order of the classes -----------------------------------------------------
+// Whole numbers that rise with the value, NaN above all, -0 equal to +0; then
+// the lowest class first.  No class has order or key 0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (x != x) return 0xFFFFFFFFu;
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return (b >> 31) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t order) {
+  if (order == 0xFFFFFFFFu) return nan_value();
+  return __uint_as_float((order >> 31) ? (order & 0x7FFFFFFFu) : ~order);
+}
+__device__ __forceinline__ uint64_t key_of(float x, int column) {
+  return ((uint64_t)order_of(x) << 32) | (0xFFFFFFFFu - (uint32_t)column);
+}
+__device__ __forceinline__ int column_of(uint64_t key) {
+  return (int)(0xFFFFFFFFu - (uint32_t)key);
+}
+
+// A wave's candidates for the top k of what it has read: every class whose
+// key lies above `bar`.  The bar never lies above the k-th best key read, and
+// a full list is cut to its k best, which raises it.
+constexpr int kListSize = 512;
+
+// lanes of one wave read in LDS what others of it wrote
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ int count_above(const uint64_t* list, int n,
+                                           uint64_t bar) {
+  int c = 0;
+  for (int i = threadIdx.x % WAVE; i < ((n + WAVE - 1) & -WAVE); i += WAVE)
+    c += __popcll(__ballot(i < n && list[i] >= bar));
+  return c;
+}
+
+// Leaves the k best of n > k distinct keys at the front of the list, in any
+// order, and returns a key that exactly they reach.  One wave.
+__device__ uint64_t cut_list(uint64_t* list, int n, int k) {
+  const int lane = threadIdx.x % WAVE;
+  wave_sync();
+  // the bits in which the keys differ, from the highest
+  uint64_t any = 0, all = ~0ull;
+  for (int i = lane; i < n; i += WAVE) {
+    any |= list[i];
+    all &= list[i];
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    any |= (uint64_t)__shfl_xor((unsigned long long)any, off, WAVE);
+    all &= (uint64_t)__shfl_xor((unsigned long long)all, off, WAVE);
+  }
+  int bit = 63 - __clzll(any ^ all);
+  uint64_t bar = bit >= 63 ? 0 : all >> (bit + 1) << (bit + 1);
+  int above = n;
+  for (; bit >= 0 && above != k; --bit) {
+    const uint64_t next = bar | 1ull << bit;
+    const int c = count_above(list, n, next);
+    if (c >= k) {
+      bar = next;
+      above = c;
+    }
+  }
+  int kept = 0;
+  for (int i = lane; i < ((n + WAVE - 1) & -WAVE); i += WAVE) {
+    const uint64_t key = i < n ? list[i] : 0;
+    const bool keep = key >= bar && i < n;
+    const uint64_t mask = __ballot(keep);
+    // written at or before where it was read, and after all lanes' reads
+    if (keep) list[kept + __popcll(mask & ((1ull << lane) - 1))] = key;
+    kept += __popcll(mask);
+  }
+  wave_sync();
+  return bar;
+}
+
+// -- log probabilities --------------------------------------------------------
+constexpr int kParts = 4;  // 16-byte loads in flight for each thread
+
+// One workgroup a part of a row (`splits` of them).  With one part the row's
+// results are written, otherwise the part's sums and its k best keys.
+template <typename E, int kThreads>
 __global__ void __launch_bounds__(kThreads)
-    label_logprobs_kernel(const T* __restrict__ logits, int64_t row_stride,
-                          int64_t rows, int classes,
-                          const int64_t* __restrict__ labels, int64_t ignore,
-                          int top, float* __restrict__ logprob,
+    label_logprobs_kernel(const typename E::Raw* __restrict__ logits,
+                          int64_t row_stride, int64_t rows, int classes,
+                          int splits, int part_size, const int64_t* __restrict__ labels,
+                          int64_t ignore, int top, float* __restrict__ logprob,
                           float* __restrict__ entropy,
                           float* __restrict__ top_logprob,
-                          int64_t* __restrict__ top_index) {
-  __shared__ float lds[kWaves];
-  __shared__ uint64_t lds_key[kWaves];
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* z = logits + row * row_stride;
-    float m = -kInf;
-    for (int c = threadIdx.x; c < classes; c += kThreads)
-      m = fmaxf(m, widen(z[c]));
-    m = block_max(m, lds);
-    const float o = origin(m);
-    float s = 0.f, t = 0.f;
-    for (int c = threadIdx.x; c < classes; c += kThreads) {
-      const float d = widen(z[c]) - o;
-      const float e = exp_of(d);
-      s += e;
-      t += e * fmaxf(d, -1e30f);
+                          int64_t* __restrict__ top_index,
+                          float* __restrict__ part_stat,
+                          uint64_t* __restrict__ part_keys) {
+  constexpr int kV = E::kVec, kWaves = kThreads / WAVE;
+  constexpr int kChunk = kThreads * kParts * kV;
+  __shared__ uint64_t lists[kWaves * kListSize];
+  __shared__ uint64_t shared_bar;
+  __shared__ int counts[kWaves];
+  __shared__ Stat stats[kWaves];
+  const int64_t row = grid_row(splits);
+  if (row >= rows) return;
+  const int part = blockIdx.x % splits;
+  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+  const typename E::Raw* z = logits + row * row_stride;
+  const int first = part * part_size;
+  const int end = min(classes, first + part_size);
+  uint64_t* list = lists + wave * kListSize;
+  int n = 0;            // candidates; the same in all lanes of a wave
+  uint64_t bar = 0;     // likewise
+  float bar_value = -kInf;
+  if (top > 0) {
+    if (threadIdx.x == 0) shared_bar = 0;
+    __syncthreads();
+  }
+
+  Stat st = Stat::none();
+  u32x4 now[kParts], next[kParts];
+#pragma unroll
+  for (int u = 0; u < kParts; ++u)
+    now[u] = load_vec<E>(z, first + (u * kThreads + (int)threadIdx.x) * kV, end);
+  for (int c0 = first; c0 < end; c0 += kChunk) {
+    const bool more = c0 + kChunk < end;
+    if (more) {
+#pragma unroll
+      for (int u = 0; u < kParts; ++u)
+        next[u] = load_vec<E>(
+            z, c0 + kChunk + (u * kThreads + (int)threadIdx.x) * kV, end);
     }
-    s = block_sum(s, lds);
-    t = block_sum(t, lds);
-    const float log_s = logf(s);
-    if (threadIdx.x == 0) {
-      entropy[row] = s == 0.f ? 0.f : log_s - t / s;
+    float best[kParts];
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) {
+      best[u] = element<E>(now[u], 0);
+#pragma unroll
+      for (int e = 1; e < kV; ++e) best[u] = fmaxf(best[u], element<E>(now[u], e));
+    }
+    float m = st.m;
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) m = fmaxf(m, best[u]);
+    st.move(m);
+    const float o = origin(m);
+#pragma unroll
+    for (int u = 0; u < kParts; ++u)
+#pragma unroll
+      for (int e = 0; e < kV; ++e) {
+        const float d = element<E>(now[u], e) - o;
+        const float x = exp_of(d);
+        st.s += x;
+        st.t += x * fmaxf(d, -1e30f);
+      }
+    if (top > 0) {
+      if (c0 == first) {
+        // The k-th best of the loads' maxima bounds the k-th best class from
+        // below: k classes at least reach it.  16 bits of its order are
+        // enough for a bar.
+        uint32_t order[kParts];
+#pragma unroll
+        for (int u = 0; u < kParts; ++u) {
+          const int at = c0 + (u * kThreads + (int)threadIdx.x) * kV;
+          order[u] = at < end ? order_of(best[u]) : 0;
+        }
+        uint32_t low = 0;
+        for (int bit = 31; bit >= 16; --bit) {
+          const uint32_t c = low | 1u << bit;
+          int reach = 0;
+#pragma unroll
+          for (int u = 0; u < kParts; ++u)
+            reach += __popcll(__ballot(order[u] >= c));
+          if (reach >= top) low = c;
+        }
+        bar = low == 0 ? 0 : ((uint64_t)low << 32) - 1;
+      }
+      // another wave's bar serves as well: it has k classes above it
+      if (lane == 0)
+        bar = atomicMax((unsigned long long*)&shared_bar, (unsigned long long)bar) > bar
+                  ? shared_bar
+                  : bar;
+      bar = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(bar >> 32)) << 32) |
+            (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)bar);
+      bar_value = bar == 0 ? -kInf : value_of((uint32_t)((bar + 1) >> 32));
+      // NaN is the greatest: where one was summed every class is looked at
+      const bool odd = st.s != st.s;
+#pragma unroll
+      for (int u = 0; u < kParts; ++u) {
+        if (__ballot(odd || !(best[u] < bar_value)) == 0) continue;
+        const int at = c0 + (u * kThreads + (int)threadIdx.x) * kV;
+#pragma unroll
+        for (int e = 0; e < kV; ++e) {
+          const float x = element<E>(now[u], e);
+          if (__ballot(!(x < bar_value)) == 0) continue;
+          const uint64_t key = at + e < end ? key_of(x, at + e) : 0;
+          uint64_t mask = __ballot(key > bar);
+          if (n + __popcll(mask) > kListSize) {
+            bar = cut_list(list, n, top) - 1;
+            n = top;
+            bar_value = value_of((uint32_t)((bar + 1) >> 32));
+            mask = __ballot(key > bar);
+          }
+          if (key > bar) list[n + __popcll(mask & ((1ull << lane) - 1))] = key;
+          n += __popcll(mask);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) now[u] = next[u];
+  }
+
+  st = block_join<kThreads>(st, stats);
+  const float log_s = logf(st.s);
+  if (top > 0) {
+    // the waves' lists, less what lies below the best bar, to one list
+    if (lane == 0) {
+      atomicMax((unsigned long long*)&shared_bar, (unsigned long long)bar);
+      counts[wave] = n;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      uint64_t* out = lists;  // filled no faster than it is read
+      const uint64_t low = shared_bar;
+      int kept = 0;
+      for (int w = 0; w < kWaves; ++w) {
+        const int have = counts[w];
+        for (int i = lane; i < ((have + WAVE - 1) & -WAVE); i += WAVE) {
+          const uint64_t key = i < have ? lists[w * kListSize + i] : 0;
+          const bool keep = key > low;
+          const uint64_t mask = __ballot(keep);
+          if (keep) out[kept + __popcll(mask & ((1ull << lane) - 1))] = key;
+          kept += __popcll(mask);
+        }
+      }
+      if (kept > top) {
+        cut_list(out, kept, top);
+        kept = top;
+      } else {
+        wave_sync();
+      }
+      for (int i = lane; i < top; i += WAVE) {
+        const uint64_t key = i < kept ? out[i] : 0;
+        if (splits > 1) {
+          part_keys[(row * splits + part) * top + i] = key;
+          continue;
+        }
+        int rank = 0;
+        for (int j = 0; j < kept; ++j) rank += out[j] > key;
+        top_index[row * top + rank] = column_of(key);
+        top_logprob[row * top + rank] =
+            log_prob(value_of((uint32_t)(key >> 32)), st.m, log_s);
+      }
+    }
+  }
+  if (threadIdx.x == 0) {
+    if (splits > 1) {
+      float* p = part_stat + (row * splits + part) * 3;
+      p[0] = st.m;
+      p[1] = st.s;
+      p[2] = st.t;
+    } else {
+      entropy[row] = st.s == 0.f ? 0.f : log_s - st.t / st.s;
       if (labels != nullptr) {
         const int64_t y = labels[row];
-        float lp = __builtin_nanf("");
+        float lp = nan_value();
         if (y == ignore)
           lp = 0.f;
         else if (y >= 0 && y < classes)
-          lp = log_prob(widen(z[y]), m, log_s);
+          lp = log_prob(E::widen(z[y]), st.m, log_s);
         logprob[row] = lp;
       }
-    }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < top; ++k) {
-      uint64_t best = 0;
-      for (int c = threadIdx.x; c < classes; c += kThreads) {
-        const uint64_t key = key_of(widen(z[c]), c);
-        if (key < last && key > best) best = key;
-      }
-      best = wave_max_key(best);
-      __syncthreads();
-      if (threadIdx.x % WAVE == 0) lds_key[threadIdx.x / WAVE] = best;
-      __syncthreads();
-      best = lds_key[0];
-#pragma unroll
-      for (int i = 1; i < kWaves; ++i) best = max(best, lds_key[i]);
-      if (threadIdx.x == 0) {
-        const uint32_t c = column_of(best);
-        top_index[row * top + k] = c;
-        top_logprob[row * top + k] = log_prob(widen(z[c]), m, log_s);
-      }
-      last = best;
     }
   }
 }
 
-// ---------------------------------------------------------------------------
-// distillation
-// ---------------------------------------------------------------------------
+// Joins a row's parts: one wave a row.
+constexpr int kMostSplits = ATOMO_LOGIT_MAX_SPLITS;
 
-// A teacher's row.
-struct Sparse {
-  float value[kTopMax];  // t, then log q
-  int column[kTopMax];   // -1: absent
-  float share[kTopMax];
-  float red[kWaves];
-  int bad;
+template <typename E>
+__global__ void __launch_bounds__(WAVE)
+    join_logprobs_kernel(const typename E::Raw* __restrict__ logits,
+                         int64_t row_stride, int64_t rows, int classes,
+                         int splits, const int64_t* __restrict__ labels, int64_t ignore,
+                         int top, float* __restrict__ logprob,
+                         float* __restrict__ entropy,
+                         float* __restrict__ top_logprob,
+                         int64_t* __restrict__ top_index,
+                         const float* __restrict__ part_stat,
+                         const uint64_t* __restrict__ part_keys) {
+  __shared__ uint64_t list[kMostSplits * ATOMO_LOGIT_TOP_MAX];
+  const int64_t row = grid_row(1);
+  if (row >= rows) return;
+  const int lane = threadIdx.x;
+  static_assert(kMostSplits <= WAVE, "a lane joins one part");
+  Stat st = Stat::none();
+  if (lane < splits) {
+    const float* p = part_stat + (row * splits + lane) * 3;
+    st = {p[0], p[1], p[2]};
+  }
+  st = wave_join(st);
+  const float log_s = logf(st.s);
+  if (top > 0) {
+    const uint64_t* keys = part_keys + row * splits * top;
+    const int all = splits * top;
+    int n = 0;
+    for (int i = lane; i < ((all + WAVE - 1) & -WAVE); i += WAVE) {
+      const uint64_t key = i < all ? keys[i] : 0;
+      const uint64_t mask = __ballot(key != 0);
+      if (key != 0) list[n + __popcll(mask & ((1ull << lane) - 1))] = key;
+      n += __popcll(mask);
+    }
+    if (n > top) {
+      cut_list(list, n, top);
+      n = top;
+    } else {
+      wave_sync();
+    }
+    for (int i = lane; i < n; i += WAVE) {
+      const uint64_t key = list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += list[j] > key;
+      top_index[row * top + rank] = column_of(key);
+      top_logprob[row * top + rank] =
+          log_prob(value_of((uint32_t)(key >> 32)), st.m, log_s);
+    }
+  }
+  if (lane == 0) {
+    entropy[row] = st.s == 0.f ? 0.f : log_s - st.t / st.s;
+    if (labels != nullptr) {
+      const int64_t y = labels[row];
+      float lp = nan_value();
+      if (y == ignore)
+        lp = 0.f;
+      else if (y >= 0 && y < classes)
+        lp = log_prob(E::widen(logits[row * row_stride + y]), st.m, log_s);
+      logprob[row] = lp;
+    }
+  }
+}
+
+// -- distillation -------------------------------------------------------------
+using Distill = AtomoDistill;
+
+// What exp(d) costs beside exp(d / tau): nothing at tau 1, a square at 2, two
+// at 4 (each a rounding of half a step), an exponential of its own elsewhere.
+enum Mode {
+  kSoftOnly = ATOMO_DISTILL_SOFT,
+  kTau1 = ATOMO_DISTILL_TAU1,
+  kTau2 = ATOMO_DISTILL_TAU2,
+  kTau4 = ATOMO_DISTILL_TAU4
 };
+
+__device__ __forceinline__ float hard_exp(int mode, float d, float soft) {
+  if (mode == kTau1) return soft;
+  if (mode == kTau2) return soft * soft;
+  if (mode == kTau4) {
+    const float s = soft * soft;
+    return s * s;
+  }
+  return exp_of(d);
+}
+
+// A teacher's row and the label in the registers of the first wave: a lane
+// holds entries lane and lane + 64.
+struct Teacher {
+  int column[2];     // -1: absent, or an earlier entry stands for its class
+  float q[2], lq[2]; // of the class: q and its logarithm
+  float z[2];        // the student's logit there
+  float sum;         // of q: 1, 0 for no entry, NaN for a wrong one
+  bool hard;         // a label counts
+  float zy;          // the student's logit at the label, NaN for a wrong one
+  int y;             // the label, -1 for a wrong one
+  bool seen;         // the label is among the entries
+
+  template <typename E>
+  __device__ void read(const Distill& a, int64_t row,
+                       const typename E::Raw* z_row, int64_t label) {
+    const int lane = threadIdx.x % WAVE;
+    float v[2];
+    bool wrong = false;
+    float m = -kInf;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = lane + h * WAVE;
+      v[h] = j < a.k ? a.values[row * a.k + j] : -kInf;
+      column[h] = -1;
+      if (v[h] != -kInf) {
+        const int64_t i = a.index[row * a.k + j];
+        if (i >= 0 && i < a.classes)
+          column[h] = (int)i;
+        else
+          wrong = true;
+      }
+      m = fmaxf(m, v[h]);
+    }
+    const float o = origin(wave_max(m));
+    float s = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s += exp_of((v[h] - o) * a.inv_tau);
+    s = wave_sum(s);
+    const float log_s = logf(s);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      lq[h] = column[h] < 0 ? -kInf : (v[h] - o) * a.inv_tau - log_s;
+      q[h] = column[h] < 0 ? 0.f : exp_of(lq[h]);
+      z[h] = column[h] < 0 ? 0.f : E::widen(z_row[column[h]]);
+    }
+    sum = s == 0.f ? 0.f : (s == s ? 1.f : s);
+    if (__ballot(wrong) != 0) sum = nan_value();
+    // entries of one class: the first stands for all
+    bool later[2] = {false, false};
+    float more[2] = {0.f, 0.f};
+    const int n = min(a.k, WAVE), n2 = a.k - n;
+    for (int j = 0; j < n; ++j) {
+      const int c = __builtin_amdgcn_readlane(column[0], j);
+      const float qj = __uint_as_float(
+          __builtin_amdgcn_readlane(__float_as_uint(q[0]), j));
+      if (column[0] == c && j != lane) {
+        later[0] |= j < lane;
+        more[0] += qj;
+      }
+      if (column[1] == c) later[1] = true;
+    }
+    for (int j = 0; j < n2; ++j) {
+      const int c = __builtin_amdgcn_readlane(column[1], j);
+      const float qj = __uint_as_float(
+          __builtin_amdgcn_readlane(__float_as_uint(q[1]), j));
+      if (column[0] == c) more[0] += qj;
+      if (column[1] == c && j != lane) {
+        later[1] |= j < lane;
+        more[1] += qj;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (column[h] >= 0 && !later[h] && more[h] > 0.f) {
+        q[h] += more[h];
+        lq[h] = logf(q[h]);
+      }
+      if (later[h]) column[h] = -1;
+    }
+    hard = a.labels != nullptr && a.weight != 1.f;
+    y = -1;
+    zy = nan_value();
+    if (hard && label >= 0 && label < a.classes) {
+      y = (int)label;
+      zy = E::widen(z_row[label]);
+    }
+    seen = __ballot(y >= 0 && (column[0] == y || column[1] == y)) != 0;
+  }
+
+  // the row's loss; all lanes of the first wave
+  __device__ float loss(const Distill& a, const Sums& st) const {
+    if (st.s == 0.f) return 0.f;  // a row of -inf only
+    const float o = origin(st.m), log_st = logf(st.t);
+    float kd = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (column[h] < 0) continue;
+      if (!(q[h] <= 0.f))
+        kd += q[h] * (lq[h] - ((z[h] - o) * a.inv_tau - log_st));
+    }
+    kd = wave_sum(kd);
+    float row = 0.f;
+    if (a.weight != 0.f)
+      row = a.weight * a.tau * a.tau * (sum != sum ? sum : kd);
+    if (hard) row += (1.f - a.weight) * (logf(st.s) - (zy - o));
+    return row;
+  }
+
+  // dz of the entries' classes and the label's within [first, end), over what
+  // the sweep wrote there; ct and c1 as in Factors
+  template <typename E>
+  __device__ void patch(const Distill& a, const Sums& st, float pt, float p1,
+                        float ct, float c1, typename E::Raw* g, int first,
+                        int end) const {
+    const float o = origin(st.m);
+    const auto put = [&](int c, float zc, float minus) {
+      if (c < first || c >= end) return;
+      const float d = zc - o;
+      const float soft = exp_of(d * a.inv_tau);
+      float x = pt * soft;
+      if (a.mode != kSoftOnly) x += p1 * hard_exp(a.mode, d, soft);
+      g[c] = E::narrow(x - minus);
+    };
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (column[h] >= 0)
+        put(column[h], z[h], ct * q[h] + (hard && column[h] == y ? c1 : 0.f));
+    if (hard && y >= 0 && !seen && threadIdx.x % WAVE == 0) put(y, zy, c1);
+  }
+};
+
+// Rows that a mean counts: all lanes of the first wave.
+__device__ __forceinline__ float inverse_count(const Distill& a) {
+  if (a.inverse != nullptr) return *a.inverse;
+  if (!a.count) return a.factor;
+  int n = 0;
+  for (int64_t i = threadIdx.x % WAVE; i < a.rows; i += WAVE)
+    n += a.labels[i] != a.ignore;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, WAVE);
+  return 1.0f / (float)(n > 0 ? n : 1);
+}
+
+template <typename E>
+__device__ __forceinline__ void add_exps(const u32x4& v, float o, float inv_tau,
+                                         int mode, Sums& st) {
+  float soft[E::kVec];
+  const float c = inv_tau * kLog2e;
+#pragma unroll
+  for (int e = 0; e < E::kVec; ++e) {
+    soft[e] = __builtin_amdgcn_exp2f((element<E>(v, e) - o) * c);
+    st.t += soft[e];
+  }
+  if (mode == kSoftOnly) return;
+  if (mode == kTau1) {
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) st.s += soft[e];
+  } else if (mode == kTau2) {
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) st.s += soft[e] * soft[e];
+  } else if (mode == kTau4) {
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) {
+      const float s = soft[e] * soft[e];
+      st.s += s * s;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) st.s += exp_of(element<E>(v, e) - o);
+  }
+}
+
+template <typename E>
+__device__ __forceinline__ void write_grad(const u32x4& v, float o,
+                                           float inv_tau, int mode, float pt,
+                                           float p1, typename E::Raw* g, int at,
+                                           int end) {
+  if (at >= end) return;
+  float x[E::kVec];
+  const float c = inv_tau * kLog2e;
+#pragma unroll
+  for (int e = 0; e < E::kVec; ++e)
+    x[e] = __builtin_amdgcn_exp2f((element<E>(v, e) - o) * c);
+  if (mode == kSoftOnly) {
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) x[e] *= pt;
+  } else if (mode == kTau1) {
+    const float p = pt + p1;
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) x[e] *= p;
+  } else if (mode == kTau2) {
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) x[e] = x[e] * (pt + p1 * x[e]);
+  } else if (mode == kTau4) {
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e) {
+      const float s = x[e] * x[e];
+      x[e] = pt * x[e] + p1 * (s * s);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E::kVec; ++e)
+      x[e] = pt * x[e] + p1 * exp_of(element<E>(v, e) - o);
+  }
+  store_vec<E>(g, at, end, x);
+}
+
+template <typename E, int kThreads>
+__device__ __forceinline__ void write_zeros(typename E::Raw* g, int first,
+                                            int end) {
+  const float zero[E::kVec] = {};
+  for (int at = first + (int)threadIdx.x * E::kVec; at < end;
+       at += kThreads * E::kVec)
+    store_vec<E>(g, at, end, zero);
+}
+
+// Loss and, where it is wanted, gradient of a row that fits a workgroup's
+// registers, kLoads 16-byte loads a thread: the logits are read once.
+template <typename E, int kThreads, int kLoads>
+__global__ void __launch_bounds__(kThreads)
+    distill_fused_kernel(Distill a) {
+  constexpr int kV = E::kVec, kWaves = kThreads / WAVE;
+  __shared__ float lds_max[kWaves];
+  __shared__ Sums lds_sums[kWaves];
+  __shared__ float lds_scale, lds_sum;
+  const int64_t row = grid_row(1);
+  if (row >= a.rows) return;
+  using Raw = typename E::Raw;
+  const Raw* z = (const Raw*)a.logits + row * a.row_stride;
+  Raw* g = (Raw*)a.grad + row * a.classes;
+  const int64_t label = a.labels ? a.labels[row] : 0;
+  if (a.labels && label == a.ignore) {
+    if (a.grad) write_zeros<E, kThreads>(g, 0, a.classes);
+    if (threadIdx.x == 0) a.row_loss[row] = 0.f;
+    return;
+  }
+  u32x4 v[kLoads];
+#pragma unroll
+  for (int r = 0; r < kLoads; ++r)
+    v[r] = load_vec<E>(z, (r * kThreads + (int)threadIdx.x) * kV, a.classes);
+  const int wave = threadIdx.x / WAVE;
+  Teacher teacher;
+  if (wave == 0) {
+    teacher.read<E>(a, row, z, label);
+    const float scale = inverse_count(a);
+    if (threadIdx.x == 0) {
+      lds_scale = scale;
+      lds_sum = teacher.sum;
+    }
+  }
+  float m = -kInf;
+#pragma unroll
+  for (int r = 0; r < kLoads; ++r)
+#pragma unroll
+    for (int e = 0; e < kV; ++e) m = fmaxf(m, element<E>(v[r], e));
+  m = wave_max(m);
+  if (threadIdx.x % WAVE == 0) lds_max[wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds_max[w]);
+  const float o = origin(m);
+  Sums st = {m, 0.f, 0.f};
+#pragma unroll
+  for (int r = 0; r < kLoads; ++r)
+    if (r * kThreads * kV < a.classes)
+      add_exps<E>(v[r], o, a.inv_tau, a.mode, st);
+  st.s = wave_sum(st.s);
+  st.t = wave_sum(st.t);
+  if (threadIdx.x % WAVE == 0) lds_sums[wave] = st;
+  __syncthreads();
+  st.s = st.t = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    st.s += lds_sums[w].s;
+    st.t += lds_sums[w].t;
+  }
+  if (a.mode == kSoftOnly) st.s = st.t;  // only whether it is 0 is asked
+  const float scale = lds_scale, q_sum = lds_sum;
+  const bool hard = a.labels != nullptr && a.weight != 1.f;
+  const float ct = a.weight == 0.f ? 0.f : a.weight * a.tau * scale;
+  float c1 = hard ? (1.f - a.weight) * scale : 0.f;
+  const float wrong =
+      hard && !(label >= 0 && label < a.classes) ? nan_value() : 0.f;
+  if (wave == 0) {
+    const float loss = teacher.loss(a, st);
+    if (threadIdx.x == 0) {
+      a.row_loss[row] = loss;
+      float* p = a.stats + row * a.splits * 3;
+      p[0] = st.m;
+      p[1] = st.s;
+      p[2] = st.t;
+    }
+  }
+  if (a.grad == nullptr) return;
+  if (st.s == 0.f) {
+    write_zeros<E, kThreads>(g, 0, a.classes);
+    return;
+  }
+  const float pt = (a.weight == 0.f ? 0.f : ct * q_sum) / st.t + wrong;
+  const float p1 = c1 / st.s;
+#pragma unroll
+  for (int r = 0; r < kLoads; ++r)
+    write_grad<E>(v[r], o, a.inv_tau, a.mode, pt, p1, g,
+                  (r * kThreads + (int)threadIdx.x) * kV, a.classes);
+  __syncthreads();
+  if (wave == 0) teacher.patch<E>(a, st, pt, p1, ct, c1, g, 0, a.classes);
+}
+
+constexpr int kSweep = 256;
+
+// The sums of a part of a row.
+template <typename E>
+__global__ void __launch_bounds__(kSweep) distill_sums_kernel(Distill a) {
+  constexpr int kV = E::kVec;
+  constexpr int kChunk = kSweep * kParts * kV;
+  __shared__ Sums lds[kSweep / WAVE];
+  const int64_t row = grid_row(a.splits);
+  if (row >= a.rows) return;
+  const int part = blockIdx.x % a.splits;
+  if (a.labels && a.labels[row] == a.ignore) return;
+  const typename E::Raw* z =
+      (const typename E::Raw*)a.logits + row * a.row_stride;
+  const int first = part * a.part_size;
+  const int end = min(a.classes, first + a.part_size);
+  Sums st = Sums::none();
+  u32x4 now[kParts], next[kParts];
+#pragma unroll
+  for (int u = 0; u < kParts; ++u)
+    now[u] = load_vec<E>(z, first + (u * kSweep + (int)threadIdx.x) * kV, end);
+  for (int c0 = first; c0 < end; c0 += kChunk) {
+    if (c0 + kChunk < end) {
+#pragma unroll
+      for (int u = 0; u < kParts; ++u)
+        next[u] = load_vec<E>(
+            z, c0 + kChunk + (u * kSweep + (int)threadIdx.x) * kV, end);
+    }
+    float m = st.m;
+#pragma unroll
+    for (int u = 0; u < kParts; ++u)
+#pragma unroll
+      for (int e = 0; e < kV; ++e) m = fmaxf(m, element<E>(now[u], e));
+    st.move(m, a.inv_tau);
+    const float o = origin(m);
+#pragma unroll
+    for (int u = 0; u < kParts; ++u)
+      add_exps<E>(now[u], o, a.inv_tau, a.mode, st);
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) now[u] = next[u];
+  }
+  st = block_join<kSweep>(st, lds, a.inv_tau);
+  if (a.mode == kSoftOnly) st.s = st.t;
+  if (threadIdx.x == 0) {
+    float* p = a.stats + (row * a.splits + part) * 3;
+    p[0] = st.m;
+    p[1] = st.s;
+    p[2] = st.t;
+  }
+}
+
+__device__ __forceinline__ Sums row_sums(const Distill& a, int64_t row) {
+  Sums st = Sums::none();
+  const int lane = threadIdx.x % WAVE;
+  if (lane < a.splits) {
+    const float* p = a.stats + (row * a.splits + lane) * 3;
+    st = {p[0], p[1], p[2]};
+  }
+  return wave_join(st, a.inv_tau);
+}
+
+// The rows' losses from their sums: one wave a row.
+template <typename E>
+__global__ void __launch_bounds__(WAVE) distill_loss_kernel(Distill a) {
+  const int64_t row = grid_row(1);
+  if (row >= a.rows) return;
+  const int64_t label = a.labels ? a.labels[row] : 0;
+  float loss = 0.f;
+  if (!(a.labels && label == a.ignore)) {
+    Teacher teacher;
+    teacher.read<E>(a, row,
+                    (const typename E::Raw*)a.logits + row * a.row_stride,
+                    label);
+    loss = teacher.loss(a, row_sums(a, row));
+  }
+  if (threadIdx.x == 0) a.row_loss[row] = loss;
+}
+
+// The gradient of a part of a row from the row's sums.
+template <typename E>
+__global__ void __launch_bounds__(kSweep) distill_grad_kernel(Distill a) {
+  constexpr int kV = E::kVec;
+  __shared__ float lds_scale, lds_sum;
+  // the forward pass wrote the gradient for an upstream one of 1
+  if (a.skip_one && *a.up == 1.f) return;
+  const int64_t row = grid_row(a.grad_splits);
+  if (row >= a.rows) return;
+  const int part = blockIdx.x % a.grad_splits;
+  using Raw = typename E::Raw;
+  const Raw* z = (const Raw*)a.logits + row * a.row_stride;
+  Raw* g = (Raw*)a.grad + row * a.classes;
+  const int first = part * a.grad_part;
+  const int end = min(a.classes, first + a.grad_part);
+  const int64_t label = a.labels ? a.labels[row] : 0;
+  if (a.labels && label == a.ignore) {
+    write_zeros<E, kSweep>(g, first, end);
+    return;
+  }
+  const Sums st = row_sums(a, row);
+  if (st.s == 0.f) {
+    write_zeros<E, kSweep>(g, first, end);
+    return;
+  }
+  const int wave = threadIdx.x / WAVE;
+  Teacher teacher;
+  if (wave == 0) {
+    teacher.read<E>(a, row, z, label);
+    const float scale = inverse_count(a) * a.up[a.up_per_row ? row : 0];
+    if (threadIdx.x == 0) {
+      lds_scale = scale;
+      lds_sum = teacher.sum;
+    }
+  }
+  __syncthreads();
+  const float scale = lds_scale, q_sum = lds_sum;
+  const float o = origin(st.m);
+  const bool hard = a.labels != nullptr && a.weight != 1.f;
+  const float ct = a.weight == 0.f ? 0.f : a.weight * a.tau * scale;
+  const float c1 = hard ? (1.f - a.weight) * scale : 0.f;
+  const float wrong =
+      hard && !(label >= 0 && label < a.classes) ? nan_value() : 0.f;
+  const float pt = (a.weight == 0.f ? 0.f : ct * q_sum) / st.t + wrong;
+  const float p1 = c1 / st.s;
+  for (int c0 = first; c0 < end; c0 += kSweep * kParts * kV) {
+    u32x4 v[kParts];
+#pragma unroll
+    for (int u = 0; u < kParts; ++u)
+      v[u] = load_vec<E>(z, c0 + (u * kSweep + (int)threadIdx.x) * kV, end);
+#pragma unroll
+    for (int u = 0; u < kParts; ++u)
+      write_grad<E>(v[u], o, a.inv_tau, a.mode, pt, p1, g,
+                    c0 + (u * kSweep + (int)threadIdx.x) * kV, end);
+  }
+  __syncthreads();
+  if (wave == 0) teacher.patch<E>(a, st, pt, p1, ct, c1, g, first, end);
+}
 
 __global__ void __launch_bounds__(1024)
     count_rows_kernel(const int64_t* __restrict__ labels, int64_t rows,
@@ -252,14 +1051,12 @@ __global__ void __launch_bounds__(1024)
 }
 
 __global__ void __launch_bounds__(1024)
-    sum_rows_kernel(const float* __restrict__ row_loss, int64_t rows,
-                    const float* __restrict__ inverse, float factor,
-                    float* __restrict__ loss) {
+    sum_rows_kernel(Distill a, float* __restrict__ loss) {
   __shared__ float lds[1024 / WAVE];
   // scaled before they are added: a mean of huge rows stays finite
-  const float each = inverse ? *inverse : factor;
+  const float each = inverse_count(a);
   float v = 0.f;
-  for (int64_t i = threadIdx.x; i < rows; i += 1024) v += row_loss[i] * each;
+  for (int64_t i = threadIdx.x; i < a.rows; i += 1024) v += a.row_loss[i] * each;
   v = wave_sum(v);
   if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = v;
   __syncthreads();
@@ -270,265 +1067,139 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// Loads the teacher's row, leaves q in `share` and the class in `column`.
-// Returns the sum of q: 1, or 0 where no entry has a finite value, or NaN.
-__device__ float load_teacher(Sparse& sp, const float* values,
-                              const int64_t* index, int k, int classes,
-                              float inv_tau) {
-  __syncthreads();
-  if (threadIdx.x == 0) sp.bad = 0;
-  float m = -kInf;
-  for (int j = threadIdx.x; j < k; j += kThreads) {
-    const float v = values[j];
-    sp.value[j] = v;
-    m = fmaxf(m, v);
-  }
-  m = block_max(m, sp.red);
-  const float o = origin(m);
-  float s = 0.f;
-  for (int j = threadIdx.x; j < k; j += kThreads) {
-    const float v = sp.value[j];
-    s += exp_of((v - o) * inv_tau);
-    int c = -1;
-    if (v != -kInf) {
-      const int64_t i = index[j];
-      if (i >= 0 && i < classes)
-        c = (int)i;
-      else
-        sp.bad = 1;
-    }
-    sp.column[j] = c;
-  }
-  s = block_sum(s, sp.red);  // its barriers also publish column and bad
-  const float log_s = logf(s);
-  for (int j = threadIdx.x; j < k; j += kThreads) {
-    const float lq = sp.column[j] < 0 ? -kInf : (sp.value[j] - o) * inv_tau - log_s;
-    sp.value[j] = lq;
-    sp.share[j] = sp.column[j] < 0 ? 0.f : exp_of(lq);
-  }
-  __syncthreads();
-  if (sp.bad) return __builtin_nanf("");
-  return s == 0.f ? 0.f : (s == s ? 1.f : s);
+// A row is split where there are too few rows to fill the card: into parts
+// of one chunk of a 256-thread workgroup at least.
+constexpr int kFill = 1024;  // workgroups: four for each of 256 CUs
+
+int splits_of(int64_t rows, int classes, int vec, int* part) {
+  if (rows < 1) rows = 1;
+  const int chunk = 256 * kParts * vec;
+  int64_t n = (kFill + rows - 1) / rows;
+  n = n < kMostSplits ? n : kMostSplits;
+  const int64_t chunks = (classes + (int64_t)chunk - 1) / chunk;
+  n = n < chunks ? n : chunks;
+  if (n < 1) n = 1;
+  const int64_t size = (chunks + n - 1) / n * chunk;
+  *part = (int)(size < classes ? size : classes);
+  return (int)((classes + size - 1) / size);
 }
 
-// q of entry j's class, or -1 where an earlier entry stands for that class
-__device__ __forceinline__ float merged_share(const Sparse& sp, int j, int k,
-                                              bool* alone) {
-  const int c = sp.column[j];
-  if (c < 0) return -1.f;
-  float q = 0.f;
-  *alone = true;
-  for (int i = 0; i < k; ++i) {
-    if (sp.column[i] != c) continue;
-    if (i < j) return -1.f;
-    if (i > j) *alone = false;
-    q += sp.share[i];
+int vec_of(int type) { return type == ATOMO_F32 ? 4 : 8; }
+
+template <typename E>
+void label_logprobs(const AtomoLogprobs& a, hipStream_t stream) {
+  using Raw = typename E::Raw;
+  const Raw* z = (const Raw*)a.logits;
+  // one wave for a row that it holds in one chunk
+  if (a.splits == 1 && a.classes <= WAVE * kParts * E::kVec) {
+    hipLaunchKernelGGL((label_logprobs_kernel<E, WAVE>), grid_of(a.rows, 1),
+                       dim3(WAVE), 0, stream, z, a.row_stride, a.rows, a.classes, 1,
+                       a.classes, a.labels, a.ignore, a.top, a.logprob,
+                       a.entropy, a.top_logprob, a.top_index, nullptr, nullptr);
+    return;
   }
-  return q;
+  hipLaunchKernelGGL((label_logprobs_kernel<E, 256>), grid_of(a.rows, a.splits),
+                     dim3(256), 0, stream, z, a.row_stride, a.rows, a.classes, a.splits,
+                     a.part_size, a.labels, a.ignore, a.top, a.logprob,
+                     a.entropy, a.top_logprob, a.top_index, a.part_stat,
+                     (uint64_t*)a.part_keys);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((join_logprobs_kernel<E>), grid_of(a.rows, 1), dim3(WAVE), 0,
+                       stream, z, a.row_stride, a.rows, a.classes, a.splits, a.labels,
+                       a.ignore, a.top, a.logprob, a.entropy, a.top_logprob,
+                       a.top_index, a.part_stat, (const uint64_t*)a.part_keys);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    distill_loss_kernel(const T* __restrict__ logits, int64_t row_stride,
-                        int64_t rows, int classes,
-                        const float* __restrict__ values,
-                        const int64_t* __restrict__ index, int k,
-                        const int64_t* __restrict__ labels, int64_t ignore,
-                        float tau, float weight, float* __restrict__ row_loss,
-                        float* __restrict__ stats) {
-  __shared__ Sparse sp;
-  __shared__ float lds[kWaves];
-  const float inv_tau = 1.0f / tau;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int64_t y = labels ? labels[row] : 0;
-    if (labels && y == ignore) {
-      if (threadIdx.x == 0) row_loss[row] = 0.f;
-      continue;
-    }
-    const T* z = logits + row * row_stride;
-    float m = -kInf;
-    for (int c = threadIdx.x; c < classes; c += kThreads)
-      m = fmaxf(m, widen(z[c]));
-    m = block_max(m, lds);
-    const float o = origin(m);
-    float s1 = 0.f, st = 0.f;
-    for (int c = threadIdx.x; c < classes; c += kThreads) {
-      const float d = widen(z[c]) - o;
-      s1 += exp_of(d);
-      st += exp_of(d * inv_tau);
-    }
-    s1 = block_sum(s1, lds);
-    st = block_sum(st, lds);
-    const float q_sum =
-        load_teacher(sp, values + row * k, index + row * k, k, classes, inv_tau);
-    const float log_st = logf(st);
-    float kd = 0.f;
-    for (int j = threadIdx.x; j < k; j += kThreads) {
-      bool alone;
-      const float q = merged_share(sp, j, k, &alone);
-      if (q > 0.f) {
-        const float lp = (widen(z[sp.column[j]]) - o) * inv_tau - log_st;
-        kd += q * ((alone ? sp.value[j] : logf(q)) - lp);
-      } else if (q != q) {
-        kd = q;
-      }
-    }
-    kd = block_sum(kd, lds);
-    if (threadIdx.x == 0) {
-      float loss = 0.f;
-      if (s1 != 0.f) {  // a row of -inf only has no loss
-        if (weight != 0.f)
-          loss = weight * tau * tau * (q_sum != q_sum ? q_sum : kd);
-        if (labels && weight != 1.f) {
-          if (y >= 0 && y < classes)
-            loss += (1.f - weight) * (logf(s1) - (widen(z[y]) - o));
-          else
-            loss = __builtin_nanf("");
-        }
-      }
-      row_loss[row] = loss;
-      stats[row * 3] = m;
-      stats[row * 3 + 1] = s1;
-      stats[row * 3 + 2] = st;
-    }
-  }
+template <typename E, int kThreads, int kLoads>
+void launch_fused(const Distill& a, hipStream_t stream) {
+  hipLaunchKernelGGL((distill_fused_kernel<E, kThreads, kLoads>), grid_of(a.rows, 1),
+                     dim3(kThreads), 0, stream, a);
 }
 
-// dz from the row's statistics.  `up` is the loss's gradient: one value, or
-// one a row.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    distill_grad_kernel(const T* __restrict__ logits, int64_t row_stride,
-                        int64_t rows, int classes,
-                        const float* __restrict__ values,
-                        const int64_t* __restrict__ index, int k,
-                        const int64_t* __restrict__ labels, int64_t ignore,
-                        float tau, float weight,
-                        const float* __restrict__ stats,
-                        const float* __restrict__ up, int up_per_row,
-                        const float* __restrict__ inverse, float factor,
-                        T* __restrict__ grad) {
-  __shared__ Sparse sp;
-  const float inv_tau = 1.0f / tau;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    T* g = grad + row * classes;
-    const int64_t y = labels ? labels[row] : 0;
-    const float m = stats[row * 3], s1 = stats[row * 3 + 1];
-    const float st = stats[row * 3 + 2];
-    if ((labels && y == ignore) || s1 == 0.f) {
-      for (int c = threadIdx.x; c < classes; c += kThreads)
-        g[c] = narrow<T>(0.f);
-      continue;
-    }
-    const T* z = logits + row * row_stride;
-    const float o = origin(m);
-    const float scale =
-        up[up_per_row ? row : 0] * (inverse ? *inverse : factor);
-    const float q_sum =
-        load_teacher(sp, values + row * k, index + row * k, k, classes, inv_tau);
-    float bad = 0.f;
-    float ct = weight == 0.f ? 0.f : weight * tau * q_sum;
-    float c1 = 0.f;
-    if (labels && weight != 1.f) {
-      c1 = 1.f - weight;
-      if (!(y >= 0 && y < classes)) bad = __builtin_nanf("");
-    }
-    const float pt = ct / st * scale + bad, p1 = c1 / s1 * scale;
-    for (int c = threadIdx.x; c < classes; c += kThreads) {
-      const float d = widen(z[c]) - o;
-      g[c] = narrow<T>(pt * exp_of(d * inv_tau) + p1 * exp_of(d));
-    }
-    __syncthreads();
-    // the sparse classes over what the sweep wrote
-    for (int j = threadIdx.x; j <= k; j += kThreads) {
-      float minus;
-      int c;
-      if (j < k) {
-        bool alone;
-        const float q = merged_share(sp, j, k, &alone);
-        if (q < 0.f) continue;
-        c = sp.column[j];
-        minus = weight * tau * q * scale;
-        if (c1 != 0.f && c == y) minus += c1 * scale;
-      } else {
-        if (c1 == 0.f || !(y >= 0 && y < classes)) continue;
-        bool seen = false;
-        for (int i = 0; i < k; ++i) seen = seen || sp.column[i] == (int)y;
-        if (seen) continue;
-        c = (int)y;
-        minus = c1 * scale;
-      }
-      const float d = widen(z[c]) - o;
-      g[c] = narrow<T>((pt * exp_of(d * inv_tau) + p1 * exp_of(d)) - minus);
-    }
-    __syncthreads();
-  }
+// The smallest workgroup whose registers hold a row: more of them share a CU,
+// and one's loads run beside another's sums.
+template <typename E>
+void distill_fused(const Distill& a, hipStream_t stream) {
+  const int loads = (a.classes + E::kVec - 1) / E::kVec;
+  if (loads <= 64)
+    launch_fused<E, 64, 1>(a, stream);
+  else if (loads <= 64 * 4)
+    launch_fused<E, 64, 4>(a, stream);
+  else if (loads <= 64 * 16)
+    launch_fused<E, 64, 16>(a, stream);
+  else if (loads <= 256 * 16)
+    launch_fused<E, 256, 16>(a, stream);
+  else if (loads <= 512 * 16)
+    launch_fused<E, 512, 16>(a, stream);
+  else
+    launch_fused<E, 1024, 16>(a, stream);
 }
 
-int grid_of(int64_t rows) { return (int)(rows < 65536 ? rows : 65536); }
+template <typename E>
+void distill_loss(const Distill& a, hipStream_t stream) {
+  hipLaunchKernelGGL((distill_sums_kernel<E>), grid_of(a.rows, a.splits),
+                     dim3(kSweep), 0, stream, a);
+  hipLaunchKernelGGL((distill_loss_kernel<E>), grid_of(a.rows, 1), dim3(WAVE), 0,
+                     stream, a);
+}
+
+template <typename E>
+void distill_grad(const Distill& a, hipStream_t stream) {
+  hipLaunchKernelGGL((distill_grad_kernel<E>), grid_of(a.rows, a.grad_splits),
+                     dim3(kSweep), 0, stream, a);
+}
 
 }  // namespace
 
-#define ATOMO_BY_TYPE(type, T, ...)                     \
-  switch (type) {                                       \
-    case ATOMO_F32: { using T = float; __VA_ARGS__; break; }          \
-    case ATOMO_BF16: { using T = __hip_bfloat16; __VA_ARGS__; break; } \
-    default: { using T = __half; __VA_ARGS__; break; }  \
+#define ATOMO_BY_TYPE(type, call)      \
+  switch (type) {                      \
+    case ATOMO_F32: call<F32>(*a, stream); break;   \
+    case ATOMO_BF16: call<BF16>(*a, stream); break; \
+    default: call<F16>(*a, stream);    \
   }
 
 extern "C" {
 
-void atomo_label_logprobs_launch(const void* logits, int type,
-                                 int64_t row_stride, int64_t rows, int classes,
-                                 const int64_t* labels, int64_t ignore,
-                                 int top, float* logprob, float* entropy,
-                                 float* top_logprob, int64_t* top_index,
-                                 hipStream_t stream) {
-  ATOMO_BY_TYPE(type, T,
-                hipLaunchKernelGGL((label_logprobs_kernel<T>), dim3(grid_of(rows)), dim3(kThreads), 0, stream,
-                    (const T*)logits, row_stride, rows, classes, labels, ignore,
-                    top, logprob, entropy, top_logprob, top_index))
+int atomo_logit_splits(int64_t rows, int classes, int type, int* part_size) {
+  return splits_of(rows, classes, vec_of(type), part_size);
+}
+
+void atomo_label_logprobs_launch(const AtomoLogprobs* a, hipStream_t stream) {
+  ATOMO_BY_TYPE(a->type, label_logprobs)
+}
+
+int atomo_distill_short(int classes, int type) {
+  return classes <= WAVE * 16 * vec_of(type);
+}
+
+int atomo_distill_fits(int64_t rows, int classes, int type) {
+  // of fewer rows each is split, so as to fill the card
+  return atomo_distill_short(classes, type) ||
+         (classes <= 1024 * 16 * vec_of(type) && rows >= 128);
 }
 
 void atomo_distill_count_launch(const int64_t* labels, int64_t rows,
                                 int64_t ignore, float* inverse,
                                 hipStream_t stream) {
-  hipLaunchKernelGGL((count_rows_kernel), dim3(1), dim3(1024), 0, stream,
-                    labels, rows, ignore, inverse);
+  hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, stream, labels,
+                     rows, ignore, inverse);
 }
 
-void atomo_distill_loss_launch(const void* logits, int type, int64_t row_stride,
-                               int64_t rows, int classes, const float* values,
-                               const int64_t* index, int k,
-                               const int64_t* labels, int64_t ignore, float tau,
-                               float weight, float* row_loss, float* stats,
-                               hipStream_t stream) {
-  ATOMO_BY_TYPE(type, T,
-                hipLaunchKernelGGL((distill_loss_kernel<T>), dim3(grid_of(rows)), dim3(kThreads), 0, stream,
-                    (const T*)logits, row_stride, rows, classes, values, index,
-                    k, labels, ignore, tau, weight, row_loss, stats))
+void atomo_distill_fused_launch(const AtomoDistill* a, hipStream_t stream) {
+  ATOMO_BY_TYPE(a->type, distill_fused)
 }
 
-void atomo_distill_sum_launch(const float* row_loss, int64_t rows,
-                              const float* inverse, float factor, float* loss,
+void atomo_distill_loss_launch(const AtomoDistill* a, hipStream_t stream) {
+  ATOMO_BY_TYPE(a->type, distill_loss)
+}
+
+void atomo_distill_sum_launch(const AtomoDistill* a, float* loss,
                               hipStream_t stream) {
-  hipLaunchKernelGGL((sum_rows_kernel), dim3(1), dim3(1024), 0, stream,
-                    row_loss, rows, inverse, factor, loss);
+  hipLaunchKernelGGL(sum_rows_kernel, dim3(1), dim3(1024), 0, stream, *a, loss);
 }
 
-void atomo_distill_grad_launch(const void* logits, int type, int64_t row_stride,
-                               int64_t rows, int classes, const float* values,
-                               const int64_t* index, int k,
-                               const int64_t* labels, int64_t ignore, float tau,
-                               float weight, const float* stats,
-                               const float* up, int up_per_row,
-                               const float* inverse, float factor, void* grad,
-                               hipStream_t stream) {
-  ATOMO_BY_TYPE(type, T,
-                hipLaunchKernelGGL((distill_grad_kernel<T>), dim3(grid_of(rows)), dim3(kThreads), 0, stream,
-                    (const T*)logits, row_stride, rows, classes, values, index,
-                    k, labels, ignore, tau, weight, stats, up, up_per_row,
-                    inverse, factor, (T*)grad))
+void atomo_distill_grad_launch(const AtomoDistill* a, hipStream_t stream) {
+  ATOMO_BY_TYPE(a->type, distill_grad)
 }
 
 }  // extern "C"
