@@ -7,7 +7,7 @@
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 
-#include <limits>
+#include <algorithm>
 
 #include "linear_kernels.h"
 #include "op_bindings.h"
@@ -44,7 +44,14 @@ int64_t row_stride(const Tensor& t) {
   return t.size(0) > 1 ? t.stride(0) : t.size(1);
 }
 
-void product(AtomoProduct a) {
+void product(AtomoProduct a, const Tensor& like) {
+  atomo_product_plan(&a);
+  Tensor partial;
+  if (a.splits > 1) {
+    partial = torch::empty({a.splits, a.nj, a.ld_part},
+                           like.options().dtype(torch::kFloat32));
+    a.partial = partial.data_ptr<float>();
+  }
   atomo_product_launch(&a, cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
@@ -61,7 +68,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA (ROCm) tensor");
     TORCH_CHECK(x.dim() == 2 && weight.dim() == 2, "x and weight must be 2-d");
     const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
-    const int64_t most = std::numeric_limits<int32_t>::max() - 1024;
+    const int64_t most = (int64_t)1 << 30;
     TORCH_CHECK(m <= most && k <= most && n <= most && k >= 1 && n >= 1,
                 "x and weight have a size that is not supported");
     check_matrix(x, x, m, k, "x");
@@ -74,7 +81,10 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     const bool by_output = act == ATOMO_ACT_RELU && !residual.defined();
     Tensor slope;
     if (train && act != ATOMO_ACT_NONE && !by_output)
-      slope = torch::empty({m, n}, x.options());
+      slope = torch::empty({m, n},
+                           x.scalar_type() == torch::kFloat32
+                               ? x.options()
+                               : x.options().dtype(torch::kInt16));
     if (m > 0) {
       AtomoProduct a{};
       a.p = weight.data_ptr();
@@ -93,7 +103,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       a.type = type_of(x);
       a.form = ATOMO_FORWARD;
       a.act = (int)act;
-      product(a);
+      product(a, x);
     }
     ctx->saved_data["train"] = train;
     ctx->saved_data["bias"] = bias.defined();
@@ -134,21 +144,30 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     Tensor dp = dy;
     const bool make_dp = slope.defined() && (want_x || want_w);
     if (make_dp || want_b) {
-      Tensor partial;
-      const int row_blocks = (int)std::min<int64_t>((m + 31) / 32, 1024);
+      AtomoLinearDp d{};
+      d.dy = dy.data_ptr();
+      d.ld_dy = row_stride(dy);
+      d.slope = slope.defined() ? slope.data_ptr() : nullptr;
+      d.by_output = ctx->saved_data["by_output"].toBool();
+      d.rows = (int)m;
+      d.columns = (int)n;
+      d.type = type;
       if (make_dp) dp = torch::empty({m, n}, x.options());
+      d.dp = make_dp ? dp.data_ptr() : nullptr;
+      // blocks of 128 rows (8 for each of 16 waves) or more, 1024 at most
+      d.block_rows = (int)std::max<int64_t>(128, (m + 1023) / 1024);
+      d.row_blocks = (int)((m + d.block_rows - 1) / d.block_rows);
+      Tensor partial;
       if (want_b) {
         db = torch::empty({n}, x.options());
-        partial = torch::empty({row_blocks, n},
-                               x.options().dtype(torch::kFloat32));
+        d.db = db.data_ptr();
+        if (d.row_blocks > 1) {
+          partial = torch::empty({d.row_blocks, n},
+                                 x.options().dtype(torch::kFloat32));
+          d.partial = partial.data_ptr<float>();
+        }
       }
-      atomo_linear_dp_launch(
-          dy.data_ptr(), row_stride(dy),
-          slope.defined() ? slope.data_ptr() : nullptr,
-          ctx->saved_data["by_output"].toBool(),
-          make_dp ? dp.data_ptr() : nullptr, want_b ? db.data_ptr() : nullptr,
-          want_b ? partial.data_ptr<float>() : nullptr, row_blocks, (int)m,
-          (int)n, type, cur_stream());
+      atomo_linear_dp_launch(&d, cur_stream());
       C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     AtomoProduct a{};
@@ -166,7 +185,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       a.nj = (int)m;
       a.nk = (int)n;
       a.form = ATOMO_GRAD_X;
-      product(a);
+      product(a, x);
     }
     if (want_w) {
       dw = torch::empty({n, k}, x.options());
@@ -176,7 +195,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       a.nj = (int)n;
       a.nk = (int)m;
       a.form = ATOMO_GRAD_W;
-      product(a);
+      product(a, x);
     }
     return {dx, dw, db, dr, Tensor(), Tensor()};
   }

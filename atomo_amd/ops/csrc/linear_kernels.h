@@ -21,6 +21,12 @@
 #define ATOMO_GRAD_X 1   // the first by its own index:  weight, dp
 #define ATOMO_GRAD_W 2   // both by their own index:     x, dp
 
+// how a product is computed: tiles of that size, or a wave for a few columns
+#define ATOMO_PLAN_64 0
+#define ATOMO_PLAN_128 1
+#define ATOMO_PLAN_256 2
+#define ATOMO_PLAN_FEW_ROWS 3
+
 // out[j][i] = act(sum_k p(i, k) q(j, k) + bias[i]) + residual[j][i]
 struct AtomoProduct {
   const void* p;
@@ -28,18 +34,28 @@ struct AtomoProduct {
   void* out;
   const void* bias;      // or null
   const void* residual;  // or null
-  void* slope;           // act'(.), or null
-  int64_t ldp, ldq, ldo, ldr;
+  void* slope;           // act'(.), or null: fp32, or 16 bits (see put_slope)
+  float* partial;        // (splits, nj, ld_part), where splits > 1
+  int64_t ldp, ldq, ldo, ldr, ld_part;
   int ni, nj, nk;
   int type, form, act;
+  int plan, splits, k_part;  // by atomo_product_plan
+};
+
+// dp = dy * slope, where dp is wanted; db, the sums of its columns, likewise.
+// Without a slope dp is dy; with `by_output` the slope is relu's output.
+struct AtomoLinearDp {
+  const void* dy;
+  const void* slope;
+  void* dp;
+  void* db;
+  float* partial;  // (row_blocks, columns), where row_blocks > 1
+  int64_t ld_dy;
+  int by_output, rows, columns, row_blocks, block_rows, type;
 };
 
 extern "C" {
+void atomo_product_plan(AtomoProduct* a);
 void atomo_product_launch(const AtomoProduct* a, hipStream_t stream);
-// dp = dy * slope where dp is wanted (slope by relu's output where
-// `by_output`), and the sums of dp's columns where db is
-void atomo_linear_dp_launch(const void* dy, int64_t ld_dy, const void* slope,
-                            int by_output, void* dp, void* db, float* partial,
-                            int row_blocks, int rows, int columns, int type,
-                            hipStream_t stream);
+void atomo_linear_dp_launch(const AtomoLinearDp* a, hipStream_t stream);
 }

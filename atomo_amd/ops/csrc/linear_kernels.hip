@@ -44,6 +44,7 @@ struct F32 {
   static constexpr int kChunk = 4;  // elements in 16 bytes
   __device__ static float widen(Raw r) { return __uint_as_float(r); }
   __device__ static Raw narrow(float f) { return __float_as_uint(f); }
+  using Slope = uint32_t;
 };
 struct BF16 {
   using Raw = uint16_t;
@@ -54,6 +55,12 @@ struct BF16 {
   __device__ static Raw narrow(float f) {
     return __builtin_bit_cast(Raw, (__bf16)f);
   }
+  __device__ static f32x16 multiply(const u32x4& p, const u32x4& q, f32x16 acc) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), acc, 0, 0,
+        0);
+  }
+  using Slope = uint16_t;
 };
 struct F16 {
   using Raw = uint16_t;
@@ -64,30 +71,36 @@ struct F16 {
   __device__ static Raw narrow(float f) {
     return __builtin_bit_cast(Raw, (_Float16)f);
   }
+  __device__ static f32x16 multiply(const u32x4& p, const u32x4& q, f32x16 acc) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), acc, 0, 0,
+        0);
+  }
+  using Slope = uint16_t;
 };
 
-template <typename E>
-__device__ __forceinline__ void multiply(const u32x4& p, const u32x4& q,
-                                         f32x16& acc);
-template <>
-__device__ __forceinline__ void multiply<BF16>(const u32x4& p, const u32x4& q,
-                                               f32x16& acc) {
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-      __builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), acc, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ void multiply<F16>(const u32x4& p, const u32x4& q,
-                                              f32x16& acc) {
-  acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-      __builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), acc, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ void multiply<F32>(const u32x4& p, const u32x4& q,
-                                              f32x16& acc) {
+// acc[i][j] += the products of 16 bytes of p's rows i and q's rows j
+template <typename E, int kI, int kJ>
+__device__ __forceinline__ void multiply(const u32x4 (&p)[kI],
+                                         const u32x4 (&q)[kJ],
+                                         f32x16 (&acc)[kI][kJ]) {
+  if constexpr (E::kChunk == 4) {
+    // neighbouring instructions add to different tiles: none waits
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(
-        __uint_as_float(p[c]), __uint_as_float(q[c]), acc, 0, 0, 0);
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < kI; ++i)
+#pragma unroll
+        for (int j = 0; j < kJ; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+              __uint_as_float(p[i][c]), __uint_as_float(q[j][c]), acc[i][j], 0,
+              0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kI; ++i)
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) acc[i][j] = E::multiply(p[i], q[j], acc[i][j]);
+  }
 }
 
 // y and dy/dh of the activation at h
@@ -124,99 +137,101 @@ __device__ __forceinline__ int slot(int row, int c) {
   return row * kRowChunks + (c ^ ((row ^ (row >> 3)) & 7));
 }
 
-// Tile of kRows rows by kRowBytes of the reduction, from memory to LDS.
+// Tile of kRows rows by kRowBytes of the reduction, from memory to LDS.  What
+// is loaded is not touched before store(), so that nothing waits for it.
 template <typename E, int kRows, int kThreads, bool kAcross>
 struct Stage {
   using Raw = typename E::Raw;
   static constexpr int kC = E::kChunk;
-  static constexpr int kK = kRowBytes / sizeof(Raw);
-  static constexpr int kVecs = kRows * kRowChunks / kThreads;
-  u32x4 v[kVecs];
+  // An operand that lies across is taken in blocks of kC k by 4 rows;
+  // neighbouring threads take neighbouring rows.
+  static constexpr int kAll = kRows / 4 * kRowChunks;
+  static constexpr int kBlocks = (kAll + kThreads - 1) / kThreads;
+  static constexpr int kVecs =
+      kAcross ? kBlocks * 4 : kRows * kRowChunks / kThreads;
+  u32x4 v[kVecs];  // across, 16-bit: v[..][2 (k % 2)..] holds four rows of a k
 
-  // `at` points at row 0, reduction 0 of the tile; rows and ks remain there
-  __device__ __forceinline__ void load(const Raw* at, int64_t ld, int rows,
-                                       int ks) {
+  __device__ static bool idle(int id) {
+    return kAll % kThreads != 0 && id >= kAll;
+  }
+
+  // All of it lies in memory, but for rows from `rows` on (a multiple of four,
+  // where it lies across): another row is read in their place, which only
+  // reaches results that nobody keeps.
+  __device__ __forceinline__ void load_whole(const Raw* at, int64_t ld,
+                                             int rows) {
+    if constexpr (!kAcross) {
+#pragma unroll
+      for (int s = 0; s < kVecs; ++s) {
+        const int id = threadIdx.x + s * kThreads;
+        const Raw* src = at + min(id / kRowChunks, rows - 1) * ld +
+                         id % kRowChunks * kC;
+        if constexpr (kC == 4)
+          v[s] = *(const u32x4_a4*)src;
+        else
+          v[s] = *(const u32x4_a2*)src;
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const int id = threadIdx.x + b * kThreads;
+        if (idle(id)) break;
+        const Raw* src = at + (int64_t)(id / (kRows / 4) * kC) * ld +
+                         min(id % (kRows / 4) * 4, rows - 4);
+#pragma unroll
+        for (int e = 0; e < kC; ++e) {
+          if constexpr (kC == 4) {
+            v[b * 4 + e] = *(const u32x4_a4*)(src + e * ld);
+          } else {
+            const u32x2 r = *(const u32x2_a2*)(src + e * ld);
+            v[b * 4 + e / 2][e % 2 * 2] = r[0];
+            v[b * 4 + e / 2][e % 2 * 2 + 1] = r[1];
+          }
+        }
+      }
+    }
+  }
+
+  // `at` points at row 0, reduction 0 of the tile; rows and ks remain there,
+  // zeros follow
+  __device__ __forceinline__ void load_edge(const Raw* at, int64_t ld, int rows,
+                                            int ks) {
+#pragma unroll
+    for (int s = 0; s < kVecs; ++s) v[s] = u32x4{0, 0, 0, 0};
     if constexpr (!kAcross) {
 #pragma unroll
       for (int s = 0; s < kVecs; ++s) {
         const int id = threadIdx.x + s * kThreads;
         const int row = id / kRowChunks, k = id % kRowChunks * kC;
-        u32x4 r = {0, 0, 0, 0};
-        if (row < rows && k < ks) {
-          const Raw* src = at + row * ld + k;
-          if (k + kC <= ks) {
-            if constexpr (sizeof(Raw) == 4)
-              r = *(const u32x4_a4*)src;
-            else
-              r = *(const u32x4_a2*)src;
-          } else {
+        if (row >= rows) continue;
+        const Raw* src = at + row * ld + k;
 #pragma unroll
-            for (int e = 0; e < kC; ++e) {
-              if (k + e < ks) {
-                if constexpr (sizeof(Raw) == 4)
-                  r[e] = src[e];
-                else
-                  r[e / 2] |= (uint32_t)src[e] << (e % 2 * 16);
-              }
-            }
-          }
+        for (int e = 0; e < kC; ++e) {
+          if (k + e >= ks) continue;
+          if constexpr (kC == 4)
+            v[s][e] = src[e];
+          else
+            v[s][e / 2] |= (uint32_t)src[e] << (e % 2 * 16);
         }
-        v[s] = r;
       }
     } else {
-      // blocks of kC k by 4 rows; neighbouring threads take neighbouring rows
-      constexpr int kBlocks = kRows / 4 * kRowChunks / kThreads;
-      static_assert(kBlocks * 4 == kVecs, "a block is four chunks");
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
         const int id = threadIdx.x + b * kThreads;
+        if (idle(id)) break;
         const int row = id % (kRows / 4) * 4, k = id / (kRows / 4) * kC;
-        if constexpr (sizeof(Raw) == 4) {
-          u32x4 in[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            u32x4 r = {0, 0, 0, 0};
-            if (k + e < ks && row < rows) {
-              const Raw* src = at + (k + e) * ld + row;
-              if (row + 4 <= rows) {
-                r = *(const u32x4_a4*)src;
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (row + i < rows) r[i] = src[i];
-              }
-            }
-            in[e] = r;
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[b * 4 + i] = u32x4{in[0][i], in[1][i], in[2][i], in[3][i]};
-        } else {
-          u32x2 in[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            u32x2 r = {0, 0};
-            if (k + e < ks && row < rows) {
-              const Raw* src = at + (k + e) * ld + row;
-              if (row + 4 <= rows) {
-                r = *(const u32x2_a2*)src;
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (row + i < rows)
-                    r[i / 2] |= (uint32_t)src[i] << (i % 2 * 16);
-              }
-            }
-            in[e] = r;
-          }
+        for (int e = 0; e < kC; ++e) {
+          if (k + e >= ks) continue;
+          const Raw* src = at + (k + e) * ld + row;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            // the low or the high halves of two k
-            const uint32_t pick = i % 2 ? 0x07060302u : 0x05040100u;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              v[b * 4 + i][e] = __builtin_amdgcn_perm(
-                  in[2 * e + 1][i / 2], in[2 * e][i / 2], pick);
+            if (row + i >= rows) continue;
+            if constexpr (kC == 4)
+              v[b * 4 + e][i] = src[i];
+            else
+              v[b * 4 + e / 2][e % 2 * 2 + i / 2] |= (uint32_t)src[i]
+                                                     << (i % 2 * 16);
           }
         }
       }
@@ -232,197 +247,525 @@ struct Stage {
       }
     } else {
 #pragma unroll
-      for (int s = 0; s < kVecs; ++s) {
-        const int id = threadIdx.x + s / 4 * kThreads;
-        tile[slot(id % (kRows / 4) * 4 + s % 4, id / (kRows / 4))] = v[s];
+      for (int b = 0; b < kBlocks; ++b) {
+        const int id = threadIdx.x + b * kThreads;
+        if (idle(id)) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u32x4 out;
+          // the low or the high halves of two k
+          const uint32_t pick = i % 2 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (kC == 4)
+              out[e] = v[b * 4 + e][i];
+            else
+              out[e] = __builtin_amdgcn_perm(v[b * 4 + e][2 + i / 2],
+                                             v[b * 4 + e][i / 2], pick);
+          }
+          tile[slot(id % (kRows / 4) * 4 + i, id / (kRows / 4))] = out;
+        }
       }
     }
   }
 };
 
-constexpr int kTile = 128;
-constexpr int kThreads = 256;
+// The slope of an activation, kept for the backward pass: fp32 beside fp32
+// operands; beside 16-bit ones a fixed point number of 2^-15 steps from -1/4
+// on, exact at 0 and 1 and 2^-16 off at most.  (Slopes lie in -0.13..1.13.  In
+// bf16 itself this rounding would weigh as much as that of dp.)
+__device__ __forceinline__ void put_slope(uint32_t* at, float s) {
+  *at = __float_as_uint(s);
+}
+__device__ __forceinline__ void put_slope(uint16_t* at, float s) {
+  *at = s != s ? 0xFFFFu : (uint16_t)((int)rintf(s * 32768.f) + 8192);
+}
+__device__ __forceinline__ float slope_of(uint32_t r) {
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ float slope_of(uint16_t r) {
+  return r == 0xFFFFu ? __builtin_nanf("")
+                      : (float)((int)r - 8192) * (1.f / 32768.f);
+}
 
-// 128 x 128 of the result by 4 waves of 64 x 64 each, tiles of 128 bytes of
-// the reduction, double-buffered in LDS (64 KB: two workgroups a CU).
-template <typename E, bool kAcrossP, bool kAcrossQ>
-__global__ void __launch_bounds__(kThreads)
-    product_kernel(AtomoProduct a, int tiles_i, int tiles_j) {
+// four neighbours of a row, at the alignment of one
+template <typename Raw>
+struct Four {
+  Raw v[4];
+} __attribute__((packed, aligned(sizeof(Raw))));
+
+// bias, activation, residual and slope on four neighbouring sums of row j
+template <typename E>
+__device__ __forceinline__ void finish(const AtomoProduct& a, int64_t j, int i,
+                                       const float (&sum)[4]) {
   using Raw = typename E::Raw;
-  __shared__ u32x4 lds[2][2][kTile * kRowChunks];
+  using Slope = typename E::Slope;
+  const int n = min(4, a.ni - i);
+  if (n <= 0) return;
+  const Raw* bias = (const Raw*)a.bias;
+  const Raw* residual = (const Raw*)a.residual + j * a.ldr + i;
+  Slope* slope = (Slope*)a.slope + j * a.ni + i;
+  Raw* out = (Raw*)a.out + j * a.ldo + i;
+  Four<Raw> y, b, r;
+  Four<Slope> s;
+  if (n == 4) {
+    if (a.bias) b = *(const Four<Raw>*)(bias + i);
+    if (a.residual) r = *(const Four<Raw>*)residual;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (e >= n) break;
+    float h = sum[e];
+    if (a.bias) h += E::widen(n == 4 ? b.v[e] : bias[i + e]);
+    float d;
+    h = activate(a.act, h, &d);
+    put_slope(&s.v[e], d);
+    if (a.residual) h += E::widen(n == 4 ? r.v[e] : residual[e]);
+    y.v[e] = E::narrow(h);
+  }
+  if (n == 4) {
+    *(Four<Raw>*)out = y;
+    if (a.slope) *(Four<Slope>*)slope = s;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+      if (e >= n) break;
+      out[e] = y.v[e];
+      if (a.slope) slope[e] = s.v[e];
+    }
+  }
+}
+
+// kI x kJ of the result by kWi x kWj waves; a tile of the reduction is 128
+// bytes of each row, double-buffered in LDS.  With several parts of the
+// reduction (`splits`) each leaves its fp32 sums for join_parts_kernel.
+template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
+          int kWj>
+__global__ void __launch_bounds__(kWi* kWj * 64)
+    product_kernel(AtomoProduct a) {
+  using Raw = typename E::Raw;
+  constexpr int kThreads = kWi * kWj * 64;
   constexpr int kK = kRowBytes / sizeof(Raw);
+  constexpr int kFi = kI / kWi / 32, kFj = kJ / kWj / 32;
+  __shared__ u32x4 lds[2][(kI + kJ) * kRowChunks];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int i0 = blockIdx.x % tiles_i * kTile;
-  const int j0 = blockIdx.x / tiles_i * kTile;
-  const int rows_i = min(a.ni - i0, kTile), rows_j = min(a.nj - j0, kTile);
-  const Raw* p = (const Raw*)a.p + (kAcrossP ? (int64_t)i0 : i0 * a.ldp);
-  const Raw* q = (const Raw*)a.q + (kAcrossQ ? (int64_t)j0 : j0 * a.ldq);
+  const int tiles_i = (a.ni + kI - 1) / kI;
+  const int tiles = tiles_i * ((a.nj + kJ - 1) / kJ);
+  const int part = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+  const int i0 = tile % tiles_i * kI, j0 = tile / tiles_i * kJ;
+  const int rows_i = min(a.ni - i0, kI), rows_j = min(a.nj - j0, kJ);
+  const int k0 = part * a.k_part, ks = min(a.nk - k0, a.k_part);
+  const Raw* p = (const Raw*)a.p +
+                 (kAcrossP ? (int64_t)k0 * a.ldp + i0 : i0 * a.ldp + k0);
+  const Raw* q = (const Raw*)a.q +
+                 (kAcrossQ ? (int64_t)k0 * a.ldq + j0 : j0 * a.ldq + k0);
   const int64_t step_p = kAcrossP ? a.ldp * kK : kK;
   const int64_t step_q = kAcrossQ ? a.ldq * kK : kK;
-  const int steps = (a.nk + kK - 1) / kK;
+  const int steps = (ks + kK - 1) / kK;
 
-  f32x16 acc[2][2] = {};
-  Stage<E, kTile, kThreads, kAcrossP> sp;
-  Stage<E, kTile, kThreads, kAcrossQ> sq;
-  sp.load(p, a.ldp, rows_i, a.nk);
-  sq.load(q, a.ldq, rows_j, a.nk);
-  sp.store(lds[0][0]);
-  sq.store(lds[0][1]);
+  // steps that load_whole() may take
+  const int whole = (kAcrossP && rows_i % 4) || (kAcrossQ && rows_j % 4)
+                        ? 0
+                        : ks / kK;
+
+  f32x16 acc[kFi][kFj] = {};
+  Stage<E, kI, kThreads, kAcrossP> sp;
+  Stage<E, kJ, kThreads, kAcrossQ> sq;
+  const auto load = [&](int s) {
+    if (s < whole) {
+      sp.load_whole(p + s * step_p, a.ldp, rows_i);
+      sq.load_whole(q + s * step_q, a.ldq, rows_j);
+    } else {
+      sp.load_edge(p + s * step_p, a.ldp, rows_i, ks - s * kK);
+      sq.load_edge(q + s * step_q, a.ldq, rows_j, ks - s * kK);
+    }
+  };
+  load(0);
+  sp.store(lds[0]);
+  sq.store(lds[0] + kI * kRowChunks);
   __syncthreads();
-  const int wi = wave % 2 * 64 + lane % 32, wj = wave / 2 * 64 + lane % 32;
+  const int wi = wave % kWi * (kI / kWi), wj = wave / kWi * (kJ / kWj);
   for (int s = 0; s < steps; ++s) {
     const bool more = s + 1 < steps;
-    if (more) {
-      sp.load(p + (s + 1) * step_p, a.ldp, rows_i, a.nk - (s + 1) * kK);
-      sq.load(q + (s + 1) * step_q, a.ldq, rows_j, a.nk - (s + 1) * kK);
-    }
-    const u32x4* tp = lds[s & 1][0];
-    const u32x4* tq = lds[s & 1][1];
+    if (more) load(s + 1);
+    const u32x4* tp = lds[s & 1];
+    const u32x4* tq = tp + kI * kRowChunks;
 #pragma unroll
     for (int c = 0; c < kRowChunks; c += 2) {
-      u32x4 fp[2], fq[2];
+      u32x4 fp[kFi], fq[kFj];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        fp[t] = tp[slot(wi + t * 32, c + lane / 32)];
-        fq[t] = tq[slot(wj + t * 32, c + lane / 32)];
-      }
+      for (int t = 0; t < kFi; ++t)
+        fp[t] = tp[slot(wi + t * 32 + lane % 32, c + lane / 32)];
 #pragma unroll
-      for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-        for (int tj = 0; tj < 2; ++tj) multiply<E>(fp[ti], fq[tj], acc[ti][tj]);
+      for (int t = 0; t < kFj; ++t)
+        fq[t] = tq[slot(wj + t * 32 + lane % 32, c + lane / 32)];
+      multiply<E>(fp, fq, acc);
     }
     if (more) {
-      sp.store(lds[(s + 1) & 1][0]);
-      sq.store(lds[(s + 1) & 1][1]);
+      u32x4* to = lds[(s + 1) & 1];
+      sp.store(to);
+      sq.store(to + kI * kRowChunks);
     }
     __syncthreads();
   }
 
   // a lane holds i = 8 g + 4 (lane / 32) + 0..3 of j = lane % 32
-  const Raw* bias = (const Raw*)a.bias;
 #pragma unroll
-  for (int ti = 0; ti < 2; ++ti)
+  for (int tj = 0; tj < kFj; ++tj) {
+    const int64_t j = j0 + wj + tj * 32 + lane % 32;
+    if (j >= a.nj) continue;
 #pragma unroll
-    for (int tj = 0; tj < 2; ++tj) {
-      const int j = j0 + wj + tj * 32;
-      if (j >= a.nj) continue;
+    for (int ti = 0; ti < kFi; ++ti)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int i = i0 + wave % 2 * 64 + ti * 32 + g * 8 + lane / 32 * 4;
+        const int i = i0 + wi + ti * 32 + g * 8 + lane / 32 * 4;
+        float sum[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (i + e >= a.ni) break;
-          float h = acc[ti][tj][g * 4 + e];
-          if (bias) h += E::widen(bias[i + e]);
-          float slope;
-          float y = activate(a.act, h, &slope);
-          if (a.slope)
-            ((Raw*)a.slope)[(int64_t)j * a.ni + i + e] = E::narrow(slope);
-          if (a.residual)
-            y += E::widen(((const Raw*)a.residual)[j * a.ldr + i + e]);
-          ((Raw*)a.out)[j * a.ldo + i + e] = E::narrow(y);
+        for (int e = 0; e < 4; ++e) sum[e] = acc[ti][tj][g * 4 + e];
+        if (a.splits == 1) {
+          finish<E>(a, j, i, sum);
+        } else {
+          // rows of a multiple of four: whole vectors
+          float* out = a.partial + ((int64_t)part * a.nj + j) * a.ld_part + i;
+          if (i < a.ni) *(float4*)out = make_float4(sum[0], sum[1], sum[2], sum[3]);
         }
       }
-    }
+  }
 }
 
-// dp and the partial column sums of a block of rows; a thread a column
+constexpr int kThreads = 256;
+
+// the parts' sums, added in order, and the epilogue; a thread four neighbours
 template <typename E>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads) join_parts_kernel(AtomoProduct a) {
+  const int64_t fours = a.ld_part / 4;
+  const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t j = id / fours;
+  const int i = (int)(id % fours) * 4;
+  if (j >= a.nj) return;
+  float sum[4] = {};
+  for (int part = 0; part < a.splits; ++part) {
+    const float4 v = *(const float4*)(a.partial +
+                                      ((int64_t)part * a.nj + j) * a.ld_part + i);
+    sum[0] += v.x;
+    sum[1] += v.y;
+    sum[2] += v.z;
+    sum[3] += v.w;
+  }
+  finish<E>(a, j, i, sum);
+}
+
+// Few rows: the weight is read once, at the memory's rate, by waves that each
+// take kN of its rows and all of x's kM; a lane takes every 64th 16 bytes.
+template <typename E, int kM, int kN>
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
+  using Raw = typename E::Raw;
+  constexpr int kC = E::kChunk;
+  const int lane = threadIdx.x % 64;
+  const int n0 = (blockIdx.x * (kThreads / 64) + (int)(threadIdx.x / 64)) * kN;
+  if (n0 >= a.ni) return;
+  const Raw* w[kN];
+  const Raw* x[kM];
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+    w[n] = (const Raw*)a.p + min(n0 + n, a.ni - 1) * a.ldp;
+#pragma unroll
+  for (int m = 0; m < kM; ++m)
+    x[m] = (const Raw*)a.q + min(m, a.nj - 1) * a.ldq;
+  float sum[kN][kM] = {};
+  const auto value = [](const u32x4& v, int e) {
+    if constexpr (kC == 4)
+      return E::widen(v[e]);
+    else
+      return E::widen((uint16_t)(v[e / 2] >> (e % 2 * 16)));
+  };
+  const auto load = [](const Raw* at) -> u32x4 {
+    if constexpr (kC == 4)
+      return *(const u32x4_a4*)at;
+    else
+      return *(const u32x4_a2*)at;
+  };
+  const int whole = a.nk / kC * kC;
+  constexpr int kUnroll = kM <= 2 ? 4 : 2;
+  int k = lane * kC;
+  for (; k + (kUnroll - 1) * 64 * kC < whole; k += kUnroll * 64 * kC) {
+    u32x4 vw[kUnroll][kN];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int n = 0; n < kN; ++n) vw[u][n] = load(w[n] + k + u * 64 * kC);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int m = 0; m < kM; ++m) {
+        const u32x4 vx = load(x[m] + k + u * 64 * kC);
+#pragma unroll
+        for (int e = 0; e < kC; ++e)
+#pragma unroll
+          for (int n = 0; n < kN; ++n)
+            sum[n][m] += value(vw[u][n], e) * value(vx, e);
+      }
+  }
+  for (; k < whole; k += 64 * kC)
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const u32x4 vw = load(w[n] + k);
+#pragma unroll
+      for (int m = 0; m < kM; ++m) {
+        const u32x4 vx = load(x[m] + k);
+#pragma unroll
+        for (int e = 0; e < kC; ++e) sum[n][m] += value(vw, e) * value(vx, e);
+      }
+    }
+  if (whole + lane < a.nk) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+#pragma unroll
+      for (int m = 0; m < kM; ++m)
+        sum[n][m] += E::widen(w[n][whole + lane]) * E::widen(x[m][whole + lane]);
+  }
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int m = 0; m < kM; ++m) {
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1)
+        sum[n][m] += __shfl_xor(sum[n][m], off, 64);
+    }
+  // lane m writes row m
+#pragma unroll
+  for (int m = 0; m < kM; ++m) {
+    if (lane != m || m >= a.nj) continue;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      if (n0 + n >= a.ni) break;
+      float h = sum[n][m], d;
+      if (a.bias) h += E::widen(((const Raw*)a.bias)[n0 + n]);
+      h = activate(a.act, h, &d);
+      if (a.slope)
+        put_slope((typename E::Slope*)a.slope + (int64_t)m * a.ni + n0 + n, d);
+      if (a.residual)
+        h += E::widen(((const Raw*)a.residual)[m * a.ldr + n0 + n]);
+      ((Raw*)a.out)[m * a.ldo + n0 + n] = E::narrow(h);
+    }
+  }
+}
+
+// dp, and the sums of the columns of a block of rows.  64 lanes take 64
+// neighbouring vectors of a row, the waves every kDpWaves-th row.
+constexpr int kDpWaves = 16;
+
+template <typename E>
+__global__ void __launch_bounds__(kDpWaves * 64)
     linear_dp_kernel(const typename E::Raw* __restrict__ dy, int64_t ld_dy,
-                     const typename E::Raw* __restrict__ slope, int by_output,
+                     const void* __restrict__ slope, int by_output,
                      typename E::Raw* __restrict__ dp,
-                     float* __restrict__ partial, int rows, int columns,
+                     float* __restrict__ partial,
+                     typename E::Raw* __restrict__ db, int rows, int columns,
                      int block_rows) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= columns) return;
+  using Raw = typename E::Raw;
+  using Slope = typename E::Slope;
+  __shared__ float lds[kDpWaves][64 * 4];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int c = (blockIdx.x * 64 + lane) * 4;
+  const int n = min(4, columns - c);
   const int first = blockIdx.y * block_rows;
   const int last = min(rows, first + block_rows);
-  float sum = 0.f;
-  for (int r = first; r < last; ++r) {
-    float d = E::widen(dy[r * ld_dy + c]);
-    if (slope) {
-      const float s = E::widen(slope[(int64_t)r * columns + c]);
-      if (by_output)
-        d = s <= 0.f ? 0.f : d;
-      else
-        d *= s;
+  float sum[4] = {};
+  if (n > 0) {
+    for (int r = first + wave; r < last; r += kDpWaves) {
+      const Raw* from = dy + r * ld_dy + c;
+      const int64_t at = (int64_t)r * columns + c;
+      Four<Raw> v, y;
+      Four<Slope> s;
+      if (n == 4) {
+        v = *(const Four<Raw>*)from;
+        if (slope && by_output) y = *(const Four<Raw>*)((const Raw*)slope + at);
+        if (slope && !by_output)
+          s = *(const Four<Slope>*)((const Slope*)slope + at);
+      } else {
+        for (int e = 0; e < n; ++e) {
+          v.v[e] = from[e];
+          if (slope && by_output) y.v[e] = ((const Raw*)slope)[at + e];
+          if (slope && !by_output) s.v[e] = ((const Slope*)slope)[at + e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e >= n) break;
+        float d = E::widen(v.v[e]);
+        if (slope && by_output)
+          d = E::widen(y.v[e]) <= 0.f ? 0.f : d;
+        else if (slope)
+          d *= slope_of(s.v[e]);
+        v.v[e] = E::narrow(d);
+        sum[e] += d;
+      }
+      if (dp && n == 4) *(Four<Raw>*)(dp + at) = v;
+      if (dp && n < 4)
+        for (int e = 0; e < n; ++e) dp[at + e] = v.v[e];
     }
-    const typename E::Raw raw = E::narrow(d);
-    if (dp) dp[(int64_t)r * columns + c] = raw;
-    sum += d;
   }
-  if (partial) partial[(int64_t)blockIdx.y * columns + c] = sum;
+  if (!partial && !db) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) lds[wave][lane * 4 + e] = sum[e];
+  __syncthreads();
+  if (threadIdx.x < 256) {
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDpWaves; ++w) all += lds[w][threadIdx.x];
+    const int column = blockIdx.x * 256 + threadIdx.x;
+    if (column < columns) {
+      if (db)
+        db[column] = E::narrow(all);
+      else
+        partial[(int64_t)blockIdx.y * columns + column] = all;
+    }
+  }
 }
 
+// the blocks' column sums, 64 columns by 16 waves
 template <typename E>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kDpWaves * 64)
     linear_db_kernel(const float* __restrict__ partial, int blocks, int columns,
                      typename E::Raw* __restrict__ db) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= columns) return;
+  __shared__ float lds[kDpWaves][64];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int c = blockIdx.x * 64 + lane;
   float sum = 0.f;
-  for (int b = 0; b < blocks; ++b) sum += partial[(int64_t)b * columns + c];
-  db[c] = E::narrow(sum);
+  if (c < columns)
+    for (int b = wave; b < blocks; b += kDpWaves)
+      sum += partial[(int64_t)b * columns + c];
+  lds[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && c < columns) {
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDpWaves; ++w) all += lds[w][lane];
+    db[c] = E::narrow(all);
+  }
+}
+
+template <typename E, int kI, int kJ, int kWi, int kWj>
+void product(const AtomoProduct& a, hipStream_t stream) {
+  const int64_t tiles = (int64_t)((a.ni + kI - 1) / kI) * ((a.nj + kJ - 1) / kJ);
+  const dim3 grid((unsigned)(tiles * a.splits)), block(kWi * kWj * 64);
+  if (a.form == ATOMO_FORWARD)
+    hipLaunchKernelGGL((product_kernel<E, false, false, kI, kJ, kWi, kWj>),
+                       grid, block, 0, stream, a);
+  else if (a.form == ATOMO_GRAD_X)
+    hipLaunchKernelGGL((product_kernel<E, true, false, kI, kJ, kWi, kWj>), grid,
+                       block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((product_kernel<E, true, true, kI, kJ, kWi, kWj>), grid,
+                       block, 0, stream, a);
+}
+
+template <typename E, int kM>
+void few_rows(const AtomoProduct& a, hipStream_t stream) {
+  constexpr int kN = 2;
+  const int per = kThreads / 64 * kN;
+  hipLaunchKernelGGL((few_rows_kernel<E, kM, kN>), dim3((a.ni + per - 1) / per),
+                     dim3(kThreads), 0, stream, a);
 }
 
 template <typename E>
 void product(const AtomoProduct& a, hipStream_t stream) {
-  const int ti = (a.ni + kTile - 1) / kTile, tj = (a.nj + kTile - 1) / kTile;
-  const dim3 grid(ti * tj), block(kThreads);
-  if (a.form == ATOMO_FORWARD)
-    hipLaunchKernelGGL((product_kernel<E, false, false>), grid, block, 0,
-                       stream, a, ti, tj);
-  else if (a.form == ATOMO_GRAD_X)
-    hipLaunchKernelGGL((product_kernel<E, true, false>), grid, block, 0, stream,
-                       a, ti, tj);
-  else
-    hipLaunchKernelGGL((product_kernel<E, true, true>), grid, block, 0, stream,
-                       a, ti, tj);
+  if (a.plan == ATOMO_PLAN_FEW_ROWS) {
+    if (a.nj <= 1)
+      few_rows<E, 1>(a, stream);
+    else if (a.nj <= 2)
+      few_rows<E, 2>(a, stream);
+    else if (a.nj <= 4)
+      few_rows<E, 4>(a, stream);
+    else
+      few_rows<E, 8>(a, stream);
+    return;
+  }
+  if (a.plan == ATOMO_PLAN_64)
+    product<E, 64, 64, 2, 2>(a, stream);
+  else if (a.plan == ATOMO_PLAN_128)
+    product<E, 128, 128, 2, 2>(a, stream);
+  else if constexpr (E::kChunk == 8)
+    product<E, 256, 256, 2, 4>(a, stream);
+  if (a.splits > 1) {
+    const int64_t fours = a.ld_part / 4 * a.nj;
+    hipLaunchKernelGGL((join_parts_kernel<E>),
+                       dim3((unsigned)((fours + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, stream, a);
+  }
 }
 
 template <typename E>
-void linear_dp(const void* dy, int64_t ld_dy, const void* slope, int by_output,
-               void* dp, void* db, float* partial, int row_blocks, int rows,
-               int columns, hipStream_t stream) {
+void linear_dp(const AtomoLinearDp& a, hipStream_t stream) {
   using Raw = typename E::Raw;
-  const int wide = (columns + kThreads - 1) / kThreads;
-  hipLaunchKernelGGL((linear_dp_kernel<E>), dim3(wide, row_blocks),
-                     dim3(kThreads), 0, stream, (const Raw*)dy, ld_dy,
-                     (const Raw*)slope, by_output, (Raw*)dp,
-                     db ? partial : nullptr, rows, columns,
-                     (rows + row_blocks - 1) / row_blocks);
-  if (db)
-    hipLaunchKernelGGL((linear_db_kernel<E>), dim3(wide), dim3(kThreads), 0,
-                       stream, partial, row_blocks, columns, (Raw*)db);
+  const bool join = a.db && a.row_blocks > 1;
+  hipLaunchKernelGGL(
+      (linear_dp_kernel<E>), dim3((a.columns + 255) / 256, a.row_blocks),
+      dim3(kDpWaves * 64), 0, stream, (const Raw*)a.dy, a.ld_dy, a.slope,
+      a.by_output, (Raw*)a.dp, join ? a.partial : nullptr,
+      join ? nullptr : (Raw*)a.db, a.rows, a.columns, a.block_rows);
+  if (join)
+    hipLaunchKernelGGL((linear_db_kernel<E>), dim3((a.columns + 63) / 64),
+                       dim3(kDpWaves * 64), 0, stream, a.partial, a.row_blocks,
+                       a.columns, (Raw*)a.db);
+}
+
+int64_t tiles_of(const AtomoProduct& a, int size) {
+  return (int64_t)((a.ni + size - 1) / size) * ((a.nj + size - 1) / size);
 }
 
 }  // namespace
 
+#define ATOMO_BY_TYPE(call)                         \
+  if (a->type == ATOMO_F32)                         \
+    call<F32>(*a, stream);                          \
+  else if (a->type == ATOMO_BF16)                   \
+    call<BF16>(*a, stream);                         \
+  else                                              \
+    call<F16>(*a, stream);
+
 extern "C" {
 
-void atomo_product_launch(const AtomoProduct* a, hipStream_t stream) {
-  if (a->type == ATOMO_F32)
-    product<F32>(*a, stream);
-  else if (a->type == ATOMO_BF16)
-    product<BF16>(*a, stream);
-  else
-    product<F16>(*a, stream);
+void atomo_product_plan(AtomoProduct* a) {
+  constexpr int kCus = 256;
+  a->splits = 1;
+  a->k_part = a->nk;
+  if (a->form == ATOMO_FORWARD && a->nj <= 8) {
+    a->plan = ATOMO_PLAN_FEW_ROWS;
+    return;
+  }
+  const int step = kRowBytes / (a->type == ATOMO_F32 ? 4 : 2);
+  const int steps = (a->nk + step - 1) / step;
+  // parts of four steps at least: below, joining costs more than it spreads
+  const int most = steps >= 8 ? steps / 4 : 1;
+  const int64_t t64 = tiles_of(*a, 64), t128 = tiles_of(*a, 128);
+  int64_t tiles = t128;
+  a->plan = ATOMO_PLAN_128;
+  if (a->type != ATOMO_F32 && tiles_of(*a, 256) >= 192) {
+    a->plan = ATOMO_PLAN_256;
+    tiles = tiles_of(*a, 256);
+  } else if (t128 * most < kCus) {
+    a->plan = ATOMO_PLAN_64;
+    tiles = t64;
+  }
+  // one workgroup a CU of the largest tiles, two of the others
+  int64_t splits = (a->plan == ATOMO_PLAN_256 ? kCus : 2 * kCus) / tiles;
+  splits = splits < most ? splits : most;
+  if (splits > 1) {
+    const int part = (int)((steps + splits - 1) / splits);
+    a->k_part = part * step;
+    a->splits = (steps + part - 1) / part;
+  }
+  a->ld_part = (a->ni + 3) / 4 * 4;
 }
 
-void atomo_linear_dp_launch(const void* dy, int64_t ld_dy, const void* slope,
-                            int by_output, void* dp, void* db, float* partial,
-                            int row_blocks, int rows, int columns, int type,
-                            hipStream_t stream) {
-  if (type == ATOMO_F32)
-    linear_dp<F32>(dy, ld_dy, slope, by_output, dp, db, partial, row_blocks,
-                   rows, columns, stream);
-  else if (type == ATOMO_BF16)
-    linear_dp<BF16>(dy, ld_dy, slope, by_output, dp, db, partial, row_blocks,
-                    rows, columns, stream);
-  else
-    linear_dp<F16>(dy, ld_dy, slope, by_output, dp, db, partial, row_blocks,
-                   rows, columns, stream);
+void atomo_product_launch(const AtomoProduct* a, hipStream_t stream) {
+  ATOMO_BY_TYPE(product)
+}
+
+void atomo_linear_dp_launch(const AtomoLinearDp* a, hipStream_t stream) {
+  ATOMO_BY_TYPE(linear_dp)
 }
 
 }  // extern "C"

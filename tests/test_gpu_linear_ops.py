@@ -108,10 +108,12 @@ def _check_near(m, k, n, dtype, activation, residual):
         err = err + U * want.abs()
     assert ((y.cpu().double() - want).abs() <= err + half * want.abs() + tiny).all()
     dp = dyd * slope
-    # the slope is rounded, and its product with dy; without an activation
-    # neither is
+    # dy times the slope is rounded; the slope is, too, to fp32, or next to
+    # 16-bit operands to 2^-15 steps; without an activation neither is
     part = 0.0 if activation == "none" else 2 * half + half * half
     dslope = 0.0 if activation == "none" else 0.9 * dh + 32 * U * (1 + h.abs())
+    if activation != "none" and dtype != F32:
+        part, dslope = half, dslope + 2.0 ** -16
     edp = dyd.abs() * (part * slope.abs() + dslope * (1 + part)) + tiny
 
     def near(got, value, error, terms, size):
