@@ -26,6 +26,7 @@
 #define ATOMO_PLAN_128 1
 #define ATOMO_PLAN_256 2
 #define ATOMO_PLAN_FEW_ROWS 3
+#define ATOMO_PLAN_TINY 4
 
 // out[j][i] = act(sum_k p(i, k) q(j, k) + bias[i]) + residual[j][i]
 struct AtomoProduct {
