@@ -5,7 +5,8 @@ launch scripts port directly, and fixes its ``type=bool`` trap
 (``--enable-gpu=`` meaning False, distributed_nn.py:70-75) by using proper
 boolean flags that ALSO accept the reference's ``--enable-gpu=<anything>``
 spelling.  New flags are additive: --optimizer, --dedicated-ps,
---shrink-freq, --checkpoint-freq, --weight-decay, --svd-backend, --overlap.
+--shrink-freq, --checkpoint-freq, --weight-decay, --svd-backend, --overlap,
+--fused-linear, --distill-*, --eval-entropy.
 """
 
 from __future__ import annotations
@@ -83,6 +84,22 @@ def add_fit_args(parser: argparse.ArgumentParser) -> argparse.ArgumentParser:
     p.add_argument("--amp", action="store_true", default=False,
                    help="bf16 autocast for forward/backward (fp32 grads, "
                         "codec and optimizer unchanged)")
+    p.add_argument("--fused-linear", action="store_true", default=False,
+                   help="fully connected layers with bias and ReLU in the "
+                        "product's kernel")
+    p.add_argument("--distill-from", type=str, default=None,
+                   help="checkpoint of a teacher: train against its top "
+                        "logits as well as the labels")
+    p.add_argument("--distill-network", type=str, default=None,
+                   help="the teacher's network (default: --network)")
+    p.add_argument("--distill-top", type=int, default=10,
+                   help="how many of the teacher's logits count (at most 128)")
+    p.add_argument("--distill-temperature", type=float, default=2.0)
+    p.add_argument("--distill-weight", type=float, default=0.9,
+                   help="of the teacher; the labels have the rest")
+    p.add_argument("--eval-entropy", action="store_true", default=False,
+                   help="evaluation also reports the mean entropy of the "
+                        "predictions")
     p.add_argument("--step-timeout", type=float, default=0.0,
                    help="abort the rank if a global step stalls this many "
                         "seconds (straggler/hang watchdog; 0 = off)")
@@ -139,6 +156,12 @@ class RunConfig:
             step_timeout=a.step_timeout,
             amp=a.amp,
             wire_dtype=a.wire_dtype,
+            fused_linear=a.fused_linear,
+            distill_from=a.distill_from,
+            distill_network=a.distill_network,
+            distill_top=a.distill_top,
+            distill_temperature=a.distill_temperature,
+            distill_weight=a.distill_weight,
         )
 
 

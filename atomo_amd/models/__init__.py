@@ -15,6 +15,7 @@ from .resnet import ResNet18, ResNet34, ResNet50, ResNet101, ResNet152
 from .vgg import vgg11, vgg11_bn, vgg13, vgg13_bn, vgg16, vgg16_bn, vgg19, vgg19_bn
 from .alexnet import AlexNet
 from .densenet import DenseNet
+from .fused import fuse_linears
 
 _ZOO = {
     "LeNet": lambda num_classes=10, in_channels=1: LeNet(num_classes, in_channels),
@@ -44,12 +45,15 @@ _ZOO = {
 }
 
 
-def build_model(name: str, num_classes: int = 10, in_channels: int = 3):
+def build_model(name: str, num_classes: int = 10, in_channels: int = 3,
+                fused_linear: bool = False):
     """Zoo dispatch mirroring build_model (sync_replicas_master_nn.py:146-171
-    / distributed_worker.py:139-164)."""
+    / distributed_worker.py:139-164).  ``fused_linear`` takes the fully
+    connected layers to ops.linear_ops (bias and ReLU in the product's kernel)."""
     if name not in _ZOO:
         raise ValueError(f"unknown network {name!r}; expected one of {sorted(_ZOO)}")
-    return _ZOO[name](num_classes=num_classes, in_channels=in_channels)
+    model = _ZOO[name](num_classes=num_classes, in_channels=in_channels)
+    return fuse_linears(model) if fused_linear else model
 
 
 def model_names():
@@ -58,6 +62,7 @@ def model_names():
 
 __all__ = [
     "build_model",
+    "fuse_linears",
     "model_names",
     "LeNet",
     "FC_NN",

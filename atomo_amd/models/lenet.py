@@ -3,9 +3,13 @@
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.linear_ops import linear_relu
+
 
 class LeNet(nn.Module):
     """Two conv + two fc; 28x28 single-channel input by default."""
+
+    linear_relus = ("fc1",)
 
     def __init__(self, num_classes: int = 10, in_channels: int = 1):
         super().__init__()
@@ -18,5 +22,5 @@ class LeNet(nn.Module):
         x = F.max_pool2d(F.relu(self.conv1(x)), 2)
         x = F.max_pool2d(F.relu(self.conv2(x)), 2)
         x = x.flatten(1)
-        x = F.relu(self.fc1(x))
+        x = linear_relu(self.fc1, x)
         return self.fc2(x)

@@ -96,6 +96,12 @@ def linear_act(
     return h.to(x.dtype)
 
 
+def linear_relu(layer: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """ReLU of a layer's output, unless the layer has it in its kernel."""
+    y = layer(x)
+    return y if getattr(layer, "activation", None) == "relu" else F.relu(y)
+
+
 class FusedLinear(nn.Linear):
     """``nn.Linear`` with its activation in the same kernel; same parameters,
     same names."""

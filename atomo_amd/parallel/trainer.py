@@ -68,6 +68,12 @@ class PSTrainer:
         comm_type: str = "Bcast",
         num_aggregate: int = 0,
         wire_dtype: str = "fp32",
+        fused_linear: bool = False,
+        distill_from: Optional[str] = None,
+        distill_network: Optional[str] = None,
+        distill_top: int = 10,
+        distill_temperature: float = 2.0,
+        distill_weight: float = 0.9,
     ):
         self.comm = comm
         self.device = device or comm.device
@@ -82,7 +88,20 @@ class PSTrainer:
             # own stream.  Model-init consistency is guaranteed separately
             # by the flat-param broadcast from rank 0 below.
             torch.manual_seed(seed + comm.rank * 1000003)
-        self.model = build_model(model_name, num_classes, in_channels).to(self.device)
+        self.model = build_model(
+            model_name, num_classes, in_channels, fused_linear
+        ).to(self.device)
+        # distillation: the workers' loss is against the top logits of a
+        # checkpoint's network (a teacher), mixed with the labels'
+        self.teacher = None
+        if distill_from:
+            self._load_teacher(
+                distill_from, distill_network or model_name, num_classes,
+                in_channels, fused_linear,
+            )
+            self.distill_top = min(int(distill_top), num_classes)
+            self.distill_temperature = float(distill_temperature)
+            self.distill_weight = float(distill_weight)
         self.flat, self.params = flatten_params(self.model)
         self.wc = WireCodec(codec, self.params, self.device, rank=comm.rank)
         self.codec = codec
@@ -312,6 +331,26 @@ class PSTrainer:
         self.comm.broadcast(self.flat, src=0)
 
     # -----------------------------------------------------------------
+    def _load_teacher(self, path, network, num_classes, in_channels, fused):
+        teacher = build_model(network, num_classes, in_channels, fused)
+        ckpt = torch.load(path, map_location="cpu", weights_only=True)
+        teacher.load_state_dict(ckpt["model"])
+        self.teacher = teacher.to(self.device).eval().requires_grad_(False)
+
+    def _loss(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+        """The worker's loss on a batch: cross entropy, or distillation."""
+        out = self.model(x)
+        if self.teacher is None:
+            return self.loss_fn(out, y)
+        from ..ops.logit_ops import distill_loss, label_logprobs
+
+        with torch.no_grad():
+            top = label_logprobs(self.teacher(x), top=self.distill_top)
+        return distill_loss(
+            out, top.top_logprob, top.top_index, y,
+            temperature=self.distill_temperature, weight=self.distill_weight,
+        )
+
     def train_step(self, x: torch.Tensor, y: torch.Tensor) -> float:
         t = self.timers
         if self.graph_whole:
@@ -371,11 +410,9 @@ class PSTrainer:
                     self.flat_grad.zero_()
                     if self.amp:
                         with torch.autocast("cuda", dtype=torch.bfloat16):
-                            out = self.model(x)
-                            loss = self.loss_fn(out, y)
+                            loss = self._loss(x, y)
                     else:
-                        out = self.model(x)
-                        loss = self.loss_fn(out, y)
+                        loss = self._loss(x, y)
                     loss.backward()
                     if self.defer_loss:
                         self._loss_tensor = loss.detach()
@@ -521,7 +558,7 @@ class PSTrainer:
         """Pre-comm half of a split-graph step: zero + fwd/bwd + encode
         on static buffers (no optimizer mutation — safe to warm-run)."""
         self.flat_grad.zero_()
-        loss = self.loss_fn(self.model(self._static_x), self._static_y)
+        loss = self._loss(self._static_x, self._static_y)
         loss.backward()
         self._static_loss = loss.detach()
         if not self.wc.reducible:
@@ -600,7 +637,7 @@ class PSTrainer:
             ok = self._graphA_step(x, y)
             if not ok:  # capture failed (graph_split now False): eager body
                 self.flat_grad.zero_()
-                loss = self.loss_fn(self.model(x), y)
+                loss = self._loss(x, y)
                 loss.backward()
                 if self.defer_loss:
                     self._loss_tensor = loss.detach()
@@ -634,7 +671,7 @@ class PSTrainer:
     def _step_body(self) -> None:
         """One full training step on static buffers (the captured body)."""
         self.flat_grad.zero_()
-        loss = self.loss_fn(self.model(self._static_x), self._static_y)
+        loss = self._loss(self._static_x, self._static_y)
         loss.backward()
         self._static_loss = loss.detach()
         if self.wc.reducible:
@@ -701,17 +738,13 @@ class PSTrainer:
                 with torch.cuda.stream(side):
                     for _ in range(3):  # warmup: MIOpen algo selection
                         self.flat_grad.zero_()
-                        loss = self.loss_fn(
-                            self.model(self._static_x), self._static_y
-                        )
+                        loss = self._loss(self._static_x, self._static_y)
                         loss.backward()
                 torch.cuda.current_stream().wait_stream(side)
                 g = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(g, capture_error_mode="thread_local"):
                     self.flat_grad.zero_()
-                    self._static_loss = self.loss_fn(
-                        self.model(self._static_x), self._static_y
-                    )
+                    self._static_loss = self._loss(self._static_x, self._static_y)
                     self._static_loss.backward()
                 self._graph = g
             except Exception as exc:  # capture-unsafe model: fall back
@@ -720,7 +753,7 @@ class PSTrainer:
                 self.use_graph = False
                 self._graph = None
                 self.flat_grad.zero_()
-                loss = self.loss_fn(self.model(x), y)
+                loss = self._loss(x, y)
                 loss.backward()
                 self.last_loss = float(loss.detach())
                 return
@@ -761,21 +794,30 @@ class PSTrainer:
 
     # -----------------------------------------------------------------
     @torch.no_grad()
-    def evaluate(self, loader, max_batches: int = 0) -> dict:
+    def evaluate(
+        self, loader, max_batches: int = 0, entropy: bool = False
+    ) -> dict:
         """On-worker eval mirroring _evaluate_model
-        (distributed_worker.py:344-370): loss + Prec@1/Prec@5."""
-        from ..utils import accuracy
+        (distributed_worker.py:344-370): loss + Prec@1/Prec@5.  With
+        ``entropy`` all of it and the mean entropy of the predictions come
+        from one pass over the logits."""
+        from ..utils import accuracy, answers
 
         self.model.eval()
-        tot, loss_sum, p1_sum, p5_sum, nb = 0, 0.0, 0.0, 0.0, 0
+        tot, loss_sum, p1_sum, p5_sum, h_sum, nb = 0, 0.0, 0.0, 0.0, 0.0, 0
         for i, (x, y) in enumerate(loader):
             if max_batches and i >= max_batches:
                 break
             x, y = x.to(self.device), y.to(self.device)
             out = self.model(x)
-            loss_sum += float(self.loss_fn(out, y)) * y.numel()
             k5 = min(5, out.shape[1])
-            p1, p5 = accuracy(out, y, topk=(1, k5))
+            if entropy:
+                loss, (p1, p5), h = answers(out, y, topk=(1, k5))
+                loss_sum += loss * y.numel()
+                h_sum += h * y.numel()
+            else:
+                loss_sum += float(self.loss_fn(out, y)) * y.numel()
+                p1, p5 = accuracy(out, y, topk=(1, k5))
             p1_sum += p1 * y.numel()
             p5_sum += p5 * y.numel()
             tot += y.numel()
@@ -783,7 +825,10 @@ class PSTrainer:
         self.model.train()
         if tot == 0:
             return {"loss": float("nan"), "prec1": 0.0, "prec5": 0.0}
-        return {"loss": loss_sum / tot, "prec1": p1_sum / tot, "prec5": p5_sum / tot}
+        res = {"loss": loss_sum / tot, "prec1": p1_sum / tot, "prec5": p5_sum / tot}
+        if entropy:
+            res["entropy"] = h_sum / tot
+        return res
 
     def save_checkpoint(self, path: Optional[str] = None) -> str:
         """torch.save to train_dir/model_step_<N> (reference

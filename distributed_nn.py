@@ -95,7 +95,7 @@ def main(argv=None):
                     rec["msg_bytes_device_total"] = dev_bytes
                 print(json.dumps(rec), flush=True)
             if a.eval_freq and step % a.eval_freq == 0 and trainer.is_worker:
-                ev = trainer.evaluate(test_loader)
+                ev = trainer.evaluate(test_loader, entropy=a.eval_entropy)
                 print(
                     json.dumps({"log": "eval", "rank": comm.rank, "step": step, **ev}),
                     flush=True,

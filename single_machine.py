@@ -45,10 +45,10 @@ def main(argv=None):
                     flush=True,
                 )
             if step >= a.max_steps:
-                ev = trainer.evaluate(test_loader)
+                ev = trainer.evaluate(test_loader, entropy=a.eval_entropy)
                 print(json.dumps({"log": "eval", "step": step, **ev}), flush=True)
                 return 0
-        ev = trainer.evaluate(test_loader)
+        ev = trainer.evaluate(test_loader, entropy=a.eval_entropy)
         print(json.dumps({"log": "eval", "epoch": epoch, **ev}), flush=True)
     return 0
 
