@@ -248,10 +248,10 @@ __device__ __forceinline__ int column_of(uint64_t key) {
   return (int)(0xFFFFFFFFu - (uint32_t)key);
 }
 
-// A wave's candidates for the top k of what it has read: every class whose
-// key lies above `bar`.  The bar never lies above the k-th best key read, and
-// a full list is cut to its k best, which raises it.
-constexpr int kListSize = 512;
+// A wave's candidates for the top k: the classes whose key lies above `bar`.
+// The bar never lies above the k-th best key read, and a full list is cut to
+// its k best, which raises it.
+constexpr int kListSize = 256;
 
 // lanes of one wave read in LDS what others of it wrote
 __device__ __forceinline__ void wave_sync() {
@@ -309,260 +309,278 @@ __device__ uint64_t cut_list(uint64_t* list, int n, int k) {
 }
 
 // -- log probabilities --------------------------------------------------------
-constexpr int kParts = 4;  // 16-byte loads in flight for each thread
+// One pass over the row makes its sums and leaves, of each thread's chunk of
+// kParts loads, the maximum in LDS: 16 bits of its order, cut off downwards.
+// The k-th best of the maxima of all loads bounds the k-th best class from
+// below, for k classes reach it; so only the few chunks (about k) that reach
+// it are read again, out of a cache, and of their classes those that do.
+constexpr int kParts = 4;    // 16-byte loads in flight for each thread
+constexpr int kChunks = 16;  // between two selections
 
-// One workgroup a part of a row (`splits` of them).  With one part the row's
-// results are written, otherwise the part's sums and its k best keys.
+// The rank-th best of a wave's maxima, cut to 16 bits.
+__device__ __forceinline__ uint32_t wave_bar(const float (&best)[kParts],
+                                             int rank) {
+  uint32_t order[kParts], low = 0;
+#pragma unroll
+  for (int u = 0; u < kParts; ++u) order[u] = order_of(best[u]);
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t c = low | 1u << bit;
+    int reach = 0;
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) reach += __popcll(__ballot(order[u] >= c));
+    if (reach >= rank) low = c;
+  }
+  return low;
+}
+
+// One row's results from its sums; one thread.
+template <typename E>
+__device__ __forceinline__ void write_row(const AtomoLogprobs& a, int64_t row,
+                                          const Stat& st, float log_s) {
+  a.entropy[row] = st.s == 0.f ? 0.f : log_s - st.t / st.s;
+  if (a.labels == nullptr) return;
+  const int64_t y = a.labels[row];
+  float lp = nan_value();
+  if (y == a.ignore)
+    lp = 0.f;
+  else if (y >= 0 && y < a.classes)
+    lp = log_prob(E::widen(((const typename E::Raw*)a.logits)[row * a.row_stride + y]),
+                  st.m, log_s);
+  a.logprob[row] = lp;
+}
+
+// Writes alternative `rank` of a row.
+__device__ __forceinline__ void write_top(const AtomoLogprobs& a, int64_t row,
+                                          int rank, uint64_t key, float m,
+                                          float log_s) {
+  a.top_index[row * a.top + rank] = column_of(key);
+  a.top_logprob[row * a.top + rank] =
+      log_prob(value_of((uint32_t)(key >> 32)), m, log_s);
+}
+
+// One workgroup a part of a row.  With one part the row's results are written,
+// otherwise the part's sums and its k best keys in order, zeros after them.
 template <typename E, int kThreads>
 __global__ void __launch_bounds__(kThreads)
-    label_logprobs_kernel(const typename E::Raw* __restrict__ logits,
-                          int64_t row_stride, int64_t rows, int classes,
-                          int splits, int part_size, const int64_t* __restrict__ labels,
-                          int64_t ignore, int top, float* __restrict__ logprob,
-                          float* __restrict__ entropy,
-                          float* __restrict__ top_logprob,
-                          int64_t* __restrict__ top_index,
-                          float* __restrict__ part_stat,
-                          uint64_t* __restrict__ part_keys) {
+    label_logprobs_kernel(AtomoLogprobs a) {
+  using Raw = typename E::Raw;
   constexpr int kV = E::kVec, kWaves = kThreads / WAVE;
   constexpr int kChunk = kThreads * kParts * kV;
+  constexpr int kOwn = kParts * kV;  // classes of a thread's chunk
+  static_assert(kOwn <= WAVE && WAVE % kOwn == 0, "a wave reads whole chunks");
   __shared__ uint64_t lists[kWaves * kListSize];
-  __shared__ uint64_t shared_bar;
+  __shared__ uint16_t tops[kChunks][kThreads];
+  __shared__ uint32_t bars[kWaves];
   __shared__ int counts[kWaves];
   __shared__ Stat stats[kWaves];
-  const int64_t row = grid_row(splits);
-  if (row >= rows) return;
-  const int part = blockIdx.x % splits;
+  const int64_t row = grid_row(a.splits);
+  if (row >= a.rows) return;
+  const int part = blockIdx.x % a.splits;
   const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-  const typename E::Raw* z = logits + row * row_stride;
-  const int first = part * part_size;
-  const int end = min(classes, first + part_size);
+  const Raw* z = (const Raw*)a.logits + row * a.row_stride;
+  const int first = part * a.part_size;
+  const int end = min(a.classes, first + a.part_size);
+  const int top = a.top;
   uint64_t* list = lists + wave * kListSize;
-  int n = 0;            // candidates; the same in all lanes of a wave
-  uint64_t bar = 0;     // likewise
-  float bar_value = -kInf;
-  if (top > 0) {
-    if (threadIdx.x == 0) shared_bar = 0;
-    __syncthreads();
-  }
+  int n = 0;         // candidates; the same in all lanes of a wave
+  uint64_t bar = 0;  // likewise
+  float best[kParts];
+#pragma unroll
+  for (int u = 0; u < kParts; ++u) best[u] = -kInf;
+  // loads that hold a class: the others have no part in the bar
+  const int filled = min(kParts * WAVE * kWaves, (end - first + kV - 1) / kV);
 
   Stat st = Stat::none();
   u32x4 now[kParts], next[kParts];
 #pragma unroll
   for (int u = 0; u < kParts; ++u)
     now[u] = load_vec<E>(z, first + (u * kThreads + (int)threadIdx.x) * kV, end);
-  for (int c0 = first; c0 < end; c0 += kChunk) {
-    const bool more = c0 + kChunk < end;
-    if (more) {
+  for (int s0 = first; s0 < end; s0 += kChunks * kChunk) {
+    int chunk = 0;
+    for (int c0 = s0; c0 < min(end, s0 + kChunks * kChunk); c0 += kChunk, ++chunk) {
+      if (c0 + kChunk < end) {
 #pragma unroll
-      for (int u = 0; u < kParts; ++u)
-        next[u] = load_vec<E>(
-            z, c0 + kChunk + (u * kThreads + (int)threadIdx.x) * kV, end);
-    }
-    float best[kParts];
-#pragma unroll
-    for (int u = 0; u < kParts; ++u) {
-      best[u] = element<E>(now[u], 0);
-#pragma unroll
-      for (int e = 1; e < kV; ++e) best[u] = fmaxf(best[u], element<E>(now[u], e));
-    }
-    float m = st.m;
-#pragma unroll
-    for (int u = 0; u < kParts; ++u) m = fmaxf(m, best[u]);
-    st.move(m);
-    const float o = origin(m);
-#pragma unroll
-    for (int u = 0; u < kParts; ++u)
-#pragma unroll
-      for (int e = 0; e < kV; ++e) {
-        const float d = element<E>(now[u], e) - o;
-        const float x = exp_of(d);
-        st.s += x;
-        st.t += x * fmaxf(d, -1e30f);
+        for (int u = 0; u < kParts; ++u)
+          next[u] = load_vec<E>(
+              z, c0 + kChunk + (u * kThreads + (int)threadIdx.x) * kV, end);
       }
-    if (top > 0) {
-      if (c0 == first) {
-        // The k-th best of the loads' maxima bounds the k-th best class from
-        // below: k classes at least reach it.  16 bits of its order are
-        // enough for a bar.
-        uint32_t order[kParts];
-#pragma unroll
-        for (int u = 0; u < kParts; ++u) {
-          const int at = c0 + (u * kThreads + (int)threadIdx.x) * kV;
-          order[u] = at < end ? order_of(best[u]) : 0;
-        }
-        uint32_t low = 0;
-        for (int bit = 31; bit >= 16; --bit) {
-          const uint32_t c = low | 1u << bit;
-          int reach = 0;
-#pragma unroll
-          for (int u = 0; u < kParts; ++u)
-            reach += __popcll(__ballot(order[u] >= c));
-          if (reach >= top) low = c;
-        }
-        bar = low == 0 ? 0 : ((uint64_t)low << 32) - 1;
-      }
-      // another wave's bar serves as well: it has k classes above it
-      if (lane == 0)
-        bar = atomicMax((unsigned long long*)&shared_bar, (unsigned long long)bar) > bar
-                  ? shared_bar
-                  : bar;
-      bar = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(bar >> 32)) << 32) |
-            (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)bar);
-      bar_value = bar == 0 ? -kInf : value_of((uint32_t)((bar + 1) >> 32));
-      // NaN is the greatest: where one was summed every class is looked at
-      const bool odd = st.s != st.s;
+      float most = -kInf;
 #pragma unroll
       for (int u = 0; u < kParts; ++u) {
-        if (__ballot(odd || !(best[u] < bar_value)) == 0) continue;
-        const int at = c0 + (u * kThreads + (int)threadIdx.x) * kV;
+        float x = element<E>(now[u], 0);
+#pragma unroll
+        for (int e = 1; e < kV; ++e) x = fmaxf(x, element<E>(now[u], e));
+        best[u] = fmaxf(best[u], x);
+        most = fmaxf(most, x);
+      }
+      st.move(fmaxf(st.m, most));
+      const float o = origin(st.m);
+#pragma unroll
+      for (int u = 0; u < kParts; ++u)
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
-          const float x = element<E>(now[u], e);
-          if (__ballot(!(x < bar_value)) == 0) continue;
-          const uint64_t key = at + e < end ? key_of(x, at + e) : 0;
-          uint64_t mask = __ballot(key > bar);
-          if (n + __popcll(mask) > kListSize) {
-            bar = cut_list(list, n, top) - 1;
-            n = top;
-            bar_value = value_of((uint32_t)((bar + 1) >> 32));
-            mask = __ballot(key > bar);
-          }
-          if (key > bar) list[n + __popcll(mask & ((1ull << lane) - 1))] = key;
-          n += __popcll(mask);
+          const float d = element<E>(now[u], e) - o;
+          const float x = exp_of(d);
+          st.s += x;
+          st.t += x * fmaxf(d, -1e30f);
         }
+      // NaN is the greatest: once one was summed every chunk is looked at
+      if (top > 0)
+        tops[chunk][threadIdx.x] =
+            st.s != st.s ? 0xFFFF : (uint16_t)(order_of(most) >> 16);
+#pragma unroll
+      for (int u = 0; u < kParts; ++u) now[u] = next[u];
+    }
+    if (top == 0) continue;
+    // each wave's share of k of the maxima: the least of the bars has k above
+    uint32_t low = 0;
+    if (filled == kParts * WAVE * kWaves)
+      low = wave_bar(best, (top + kWaves - 1) / kWaves);
+    else if (kWaves == 1 && filled >= top)
+      low = wave_bar(best, top);
+    if (kWaves > 1) {
+      __syncthreads();
+      if (lane == 0) bars[wave] = low;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) low = min(low, bars[w]);
+    }
+    if (low != 0) {
+      const uint64_t at_least = ((uint64_t)low << 32) - 1;
+      bar = at_least > bar ? at_least : bar;
+    }
+    wave_sync();
+    for (int c = 0; c < chunk; ++c) {
+      uint64_t hits = __ballot(tops[c][threadIdx.x] >= (uint32_t)((bar + 1) >> 48));
+      while (hits != 0) {
+        // the next chunks that reach the bar, a lane for each of their classes
+        int who = -1;
+#pragma unroll
+        for (int g = 0; g < WAVE / kOwn; ++g) {
+          const int bit = hits ? __builtin_ctzll(hits) : -1;
+          if (lane / kOwn == g) who = bit;
+          hits &= hits - 1;
+        }
+        const int own = lane % kOwn;
+        const int at = s0 + c * kChunk +
+                       (own / kV * kThreads + wave * WAVE + who) * kV + own % kV;
+        const bool there = who >= 0 && at < end;
+        const uint64_t key = there ? key_of(E::widen(z[at]), at) : 0;
+        uint64_t mask = __ballot(key > bar);
+        if (n + __popcll(mask) > kListSize) {
+          bar = cut_list(list, n, top) - 1;
+          n = top;
+          mask = __ballot(key > bar);
+        }
+        if (key > bar) list[n + __popcll(mask & ((1ull << lane) - 1))] = key;
+        n += __popcll(mask);
       }
     }
-#pragma unroll
-    for (int u = 0; u < kParts; ++u) now[u] = next[u];
+    if (kWaves > 1) __syncthreads();  // `tops` and `bars` are written again
   }
 
   st = block_join<kThreads>(st, stats);
   const float log_s = logf(st.s);
   if (top > 0) {
-    // the waves' lists, less what lies below the best bar, to one list
-    if (lane == 0) {
-      atomicMax((unsigned long long*)&shared_bar, (unsigned long long)bar);
-      counts[wave] = n;
-    }
+    if (lane == 0) counts[wave] = n;
     __syncthreads();
-    if (wave == 0) {
-      uint64_t* out = lists;  // filled no faster than it is read
-      const uint64_t low = shared_bar;
-      int kept = 0;
-      for (int w = 0; w < kWaves; ++w) {
-        const int have = counts[w];
-        for (int i = lane; i < ((have + WAVE - 1) & -WAVE); i += WAVE) {
-          const uint64_t key = i < have ? lists[w * kListSize + i] : 0;
-          const bool keep = key > low;
-          const uint64_t mask = __ballot(keep);
-          if (keep) out[kept + __popcll(mask & ((1ull << lane) - 1))] = key;
-          kept += __popcll(mask);
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all += counts[w];
+    if (all > kListSize) {
+      // into one list, filled no faster than it is read, and cut
+      if (wave == 0) {
+        int kept = counts[0];
+        for (int w = 1; w < kWaves; ++w) {
+          const int have = counts[w];
+          for (int i = lane; i < ((have + WAVE - 1) & -WAVE); i += WAVE) {
+            const uint64_t key = i < have ? lists[w * kListSize + i] : 0;
+            if (i < have) lists[kept + i] = key;
+          }
+          kept += have;
         }
+        cut_list(lists, kept, top);
+        if (lane < kWaves) counts[lane] = lane == 0 ? top : 0;
       }
-      if (kept > top) {
-        cut_list(out, kept, top);
-        kept = top;
-      } else {
-        wave_sync();
-      }
-      for (int i = lane; i < top; i += WAVE) {
-        const uint64_t key = i < kept ? out[i] : 0;
-        if (splits > 1) {
-          part_keys[(row * splits + part) * top + i] = key;
-          continue;
-        }
-        int rank = 0;
-        for (int j = 0; j < kept; ++j) rank += out[j] > key;
-        top_index[row * top + rank] = column_of(key);
-        top_logprob[row * top + rank] =
-            log_prob(value_of((uint32_t)(key >> 32)), st.m, log_s);
-      }
+      __syncthreads();
     }
+    // a key's rank is the number of greater ones
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all += counts[w];
+    for (int i = threadIdx.x; i < all; i += kThreads) {
+      int w = 0, j = i;
+      while (j >= counts[w]) j -= counts[w++];
+      const uint64_t key = lists[w * kListSize + j];
+      int rank = 0;
+      for (w = 0; w < kWaves; ++w)
+        for (j = 0; j < counts[w]; ++j) rank += lists[w * kListSize + j] > key;
+      if (rank >= top) continue;
+      if (a.splits > 1)
+        a.part_keys[(row * a.splits + part) * top + rank] = (int64_t)key;
+      else
+        write_top(a, row, rank, key, st.m, log_s);
+    }
+    if (a.splits > 1)
+      for (int i = all + threadIdx.x; i < top; i += kThreads)
+        a.part_keys[(row * a.splits + part) * top + i] = 0;
   }
   if (threadIdx.x == 0) {
-    if (splits > 1) {
-      float* p = part_stat + (row * splits + part) * 3;
+    if (a.splits > 1) {
+      float* p = a.part_stat + (row * a.splits + part) * 3;
       p[0] = st.m;
       p[1] = st.s;
       p[2] = st.t;
     } else {
-      entropy[row] = st.s == 0.f ? 0.f : log_s - st.t / st.s;
-      if (labels != nullptr) {
-        const int64_t y = labels[row];
-        float lp = nan_value();
-        if (y == ignore)
-          lp = 0.f;
-        else if (y >= 0 && y < classes)
-          lp = log_prob(E::widen(z[y]), st.m, log_s);
-        logprob[row] = lp;
-      }
+      write_row<E>(a, row, st, log_s);
     }
   }
 }
 
-// Joins a row's parts: one wave a row.
+// Joins a row's parts: one workgroup a row.  A part's last key, where it has
+// k, is a bar for all of them.
 constexpr int kMostSplits = ATOMO_LOGIT_MAX_SPLITS;
+constexpr int kJoin = 256;
 
 template <typename E>
-__global__ void __launch_bounds__(WAVE)
-    join_logprobs_kernel(const typename E::Raw* __restrict__ logits,
-                         int64_t row_stride, int64_t rows, int classes,
-                         int splits, const int64_t* __restrict__ labels, int64_t ignore,
-                         int top, float* __restrict__ logprob,
-                         float* __restrict__ entropy,
-                         float* __restrict__ top_logprob,
-                         int64_t* __restrict__ top_index,
-                         const float* __restrict__ part_stat,
-                         const uint64_t* __restrict__ part_keys) {
+__global__ void __launch_bounds__(kJoin)
+    join_logprobs_kernel(AtomoLogprobs a) {
   __shared__ uint64_t list[kMostSplits * ATOMO_LOGIT_TOP_MAX];
-  const int64_t row = grid_row(1);
-  if (row >= rows) return;
-  const int lane = threadIdx.x;
+  __shared__ int count;
   static_assert(kMostSplits <= WAVE, "a lane joins one part");
+  const int64_t row = grid_row(1);
+  if (row >= a.rows) return;
+  const int lane = threadIdx.x % WAVE, top = a.top;
+  const uint64_t* keys = (const uint64_t*)a.part_keys + row * a.splits * top;
   Stat st = Stat::none();
-  if (lane < splits) {
-    const float* p = part_stat + (row * splits + lane) * 3;
+  uint64_t bar = 1;
+  if (lane < a.splits) {
+    const float* p = a.part_stat + (row * a.splits + lane) * 3;
     st = {p[0], p[1], p[2]};
+    if (top > 0) bar = max(bar, keys[lane * top + top - 1]);
   }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+    bar = max(bar, (uint64_t)__shfl_xor((unsigned long long)bar, off, WAVE));
   st = wave_join(st);
   const float log_s = logf(st.s);
-  if (top > 0) {
-    const uint64_t* keys = part_keys + row * splits * top;
-    const int all = splits * top;
-    int n = 0;
-    for (int i = lane; i < ((all + WAVE - 1) & -WAVE); i += WAVE) {
-      const uint64_t key = i < all ? keys[i] : 0;
-      const uint64_t mask = __ballot(key != 0);
-      if (key != 0) list[n + __popcll(mask & ((1ull << lane) - 1))] = key;
-      n += __popcll(mask);
-    }
-    if (n > top) {
-      cut_list(list, n, top);
-      n = top;
-    } else {
-      wave_sync();
-    }
-    for (int i = lane; i < n; i += WAVE) {
-      const uint64_t key = list[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += list[j] > key;
-      top_index[row * top + rank] = column_of(key);
-      top_logprob[row * top + rank] =
-          log_prob(value_of((uint32_t)(key >> 32)), st.m, log_s);
-    }
+  if (threadIdx.x == 0) {
+    count = 0;
+    write_row<E>(a, row, st, log_s);
   }
-  if (lane == 0) {
-    entropy[row] = st.s == 0.f ? 0.f : log_s - st.t / st.s;
-    if (labels != nullptr) {
-      const int64_t y = labels[row];
-      float lp = nan_value();
-      if (y == ignore)
-        lp = 0.f;
-      else if (y >= 0 && y < classes)
-        lp = log_prob(E::widen(logits[row * row_stride + y]), st.m, log_s);
-      logprob[row] = lp;
-    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.splits * top; i += kJoin) {
+    const uint64_t key = keys[i];
+    if (key >= bar) list[atomicAdd(&count, 1)] = key;
+  }
+  __syncthreads();
+  // keys are distinct: their order in the list does not matter
+  const int n = count;
+  for (int i = threadIdx.x; i < n; i += kJoin) {
+    const uint64_t key = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > key;
+    if (rank < top) write_top(a, row, rank, key, st.m, log_s);
   }
 }
 
@@ -1088,26 +1106,17 @@ int vec_of(int type) { return type == ATOMO_F32 ? 4 : 8; }
 
 template <typename E>
 void label_logprobs(const AtomoLogprobs& a, hipStream_t stream) {
-  using Raw = typename E::Raw;
-  const Raw* z = (const Raw*)a.logits;
   // one wave for a row that it holds in one chunk
   if (a.splits == 1 && a.classes <= WAVE * kParts * E::kVec) {
     hipLaunchKernelGGL((label_logprobs_kernel<E, WAVE>), grid_of(a.rows, 1),
-                       dim3(WAVE), 0, stream, z, a.row_stride, a.rows, a.classes, 1,
-                       a.classes, a.labels, a.ignore, a.top, a.logprob,
-                       a.entropy, a.top_logprob, a.top_index, nullptr, nullptr);
+                       dim3(WAVE), 0, stream, a);
     return;
   }
   hipLaunchKernelGGL((label_logprobs_kernel<E, 256>), grid_of(a.rows, a.splits),
-                     dim3(256), 0, stream, z, a.row_stride, a.rows, a.classes, a.splits,
-                     a.part_size, a.labels, a.ignore, a.top, a.logprob,
-                     a.entropy, a.top_logprob, a.top_index, a.part_stat,
-                     (uint64_t*)a.part_keys);
+                     dim3(256), 0, stream, a);
   if (a.splits > 1)
-    hipLaunchKernelGGL((join_logprobs_kernel<E>), grid_of(a.rows, 1), dim3(WAVE), 0,
-                       stream, z, a.row_stride, a.rows, a.classes, a.splits, a.labels,
-                       a.ignore, a.top, a.logprob, a.entropy, a.top_logprob,
-                       a.top_index, a.part_stat, (const uint64_t*)a.part_keys);
+    hipLaunchKernelGGL((join_logprobs_kernel<E>), grid_of(a.rows, 1),
+                       dim3(kJoin), 0, stream, a);
 }
 
 template <typename E, int kThreads, int kLoads>
