@@ -81,6 +81,10 @@ __device__ __forceinline__ float element(const u32x4& v, int e) {
     return E::widen((uint16_t)(v[e / 2] >> (e % 2 * 16)));
 }
 
+// Keeps the compiler from holding the widened elements of `v` over a pass: to
+// widen them again costs less than the registers.
+__device__ __forceinline__ void forget(u32x4& v) { asm("" : "+v"(v)); }
+
 // 16 bytes from element `at` on; from `end` on, -inf
 template <typename E>
 __device__ __forceinline__ u32x4 load_vec(const typename E::Raw* z, int at,
@@ -538,7 +542,8 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Joins a row's parts: one workgroup a row.  A part's last key, where it has
-// k, is a bar for all of them.
+// k, is a bar for all of them; so is the least of the parts' d-th keys, where
+// d keys of each are k together, and mostly the higher one.
 constexpr int kMostSplits = ATOMO_LOGIT_MAX_SPLITS;
 constexpr int kJoin = 256;
 
@@ -553,15 +558,22 @@ __global__ void __launch_bounds__(kJoin)
   const int lane = threadIdx.x % WAVE, top = a.top;
   const uint64_t* keys = (const uint64_t*)a.part_keys + row * a.splits * top;
   Stat st = Stat::none();
-  uint64_t bar = 1;
+  const int share = (top + a.splits - 1) / a.splits;
+  uint64_t bar = 1, least = ~0ull;
   if (lane < a.splits) {
     const float* p = a.part_stat + (row * a.splits + lane) * 3;
     st = {p[0], p[1], p[2]};
-    if (top > 0) bar = max(bar, keys[lane * top + top - 1]);
+    if (top > 0) {
+      bar = max(bar, keys[lane * top + top - 1]);
+      least = keys[lane * top + share - 1];
+    }
   }
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
+  for (int off = 32; off > 0; off >>= 1) {
     bar = max(bar, (uint64_t)__shfl_xor((unsigned long long)bar, off, WAVE));
+    least = min(least, (uint64_t)__shfl_xor((unsigned long long)least, off, WAVE));
+  }
+  bar = max(bar, least);
   st = wave_join(st);
   const float log_s = logf(st.s);
   if (threadIdx.x == 0) {
@@ -609,8 +621,9 @@ __device__ __forceinline__ float hard_exp(int mode, float d, float soft) {
 // A teacher's row and the label in the registers of the first wave: a lane
 // holds entries lane and lane + 64.
 struct Teacher {
+  int64_t at[2];     // as given
   int column[2];     // -1: absent, or an earlier entry stands for its class
-  float q[2], lq[2]; // of the class: q and its logarithm
+  float q[2], lq[2]; // of the class: q and its logarithm (first, the value)
   float z[2];        // the student's logit there
   float sum;         // of q: 1, 0 for no entry, NaN for a wrong one
   bool hard;         // a label counts
@@ -618,63 +631,77 @@ struct Teacher {
   int y;             // the label, -1 for a wrong one
   bool seen;         // the label is among the entries
 
-  template <typename E>
-  __device__ void read(const Distill& a, int64_t row,
-                       const typename E::Raw* z_row, int64_t label) {
+  // Reads a row's entries, all lanes of the first wave; nothing waits for them.
+  __device__ void fetch(const Distill& a, int64_t row) {
     const int lane = threadIdx.x % WAVE;
-    float v[2];
-    bool wrong = false;
-    float m = -kInf;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int j = lane + h * WAVE;
-      v[h] = j < a.k ? a.values[row * a.k + j] : -kInf;
-      column[h] = -1;
-      if (v[h] != -kInf) {
-        const int64_t i = a.index[row * a.k + j];
-        if (i >= 0 && i < a.classes)
-          column[h] = (int)i;
-        else
-          wrong = true;
-      }
-      m = fmaxf(m, v[h]);
+      lq[h] = j < a.k ? a.values[row * a.k + j] : -kInf;
+      at[h] = j < a.k ? a.index[row * a.k + j] : -1;
     }
-    const float o = origin(wave_max(m));
-    float s = 0.f;
+  }
+
+  template <typename E>
+  __device__ void read(const Distill& a, const typename E::Raw* z_row,
+                       int64_t label) {
+    const int lane = threadIdx.x % WAVE;
+    bool wrong = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) s += exp_of((v[h] - o) * a.inv_tau);
-    s = wave_sum(s);
+    for (int h = 0; h < 2; ++h) {
+      const bool there = lq[h] != -kInf, in = at[h] >= 0 && at[h] < a.classes;
+      wrong |= there && !in;
+      column[h] = there && in ? (int)at[h] : -1;
+      // used with the sums only, long after
+      z[h] = column[h] < 0 ? 0.f : E::widen(z_row[column[h]]);
+    }
+    hard = a.labels != nullptr && a.weight != 1.f;
+    y = -1;
+    zy = nan_value();
+    if (hard && label >= 0 && label < a.classes) {
+      y = (int)label;
+      zy = E::widen(z_row[label]);
+    }
+    const float o = origin(wave_max(fmaxf(lq[0], lq[1])));
+    const float s = wave_sum(exp_of((lq[0] - o) * a.inv_tau) +
+                             exp_of((lq[1] - o) * a.inv_tau));
     const float log_s = logf(s);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      lq[h] = column[h] < 0 ? -kInf : (v[h] - o) * a.inv_tau - log_s;
+      lq[h] = column[h] < 0 ? -kInf : (lq[h] - o) * a.inv_tau - log_s;
       q[h] = column[h] < 0 ? 0.f : exp_of(lq[h]);
-      z[h] = column[h] < 0 ? 0.f : E::widen(z_row[column[h]]);
     }
     sum = s == 0.f ? 0.f : (s == s ? 1.f : s);
     if (__ballot(wrong) != 0) sum = nan_value();
-    // entries of one class: the first stands for all
+    // is a class there twice?
+    bool twice = false;
+    for (int d = 1; d <= WAVE / 2; ++d)
+      twice |= column[0] >= 0 &&
+               column[0] == __shfl(column[0], (lane + d) % WAVE, WAVE);
+    if (a.k > WAVE)
+      for (int d = 0; d < WAVE; ++d) {
+        const int c = __shfl(column[1], (lane + d) % WAVE, WAVE);
+        twice |= c >= 0 && (c == column[0] || (d > 0 && c == column[1]));
+      }
+    if (__ballot(twice) != 0) merge(a);
+    seen = __ballot(y >= 0 && (column[0] == y || column[1] == y)) != 0;
+  }
+
+  // entries of one class: the first stands for all
+  __device__ void merge(const Distill& a) {
+    const int lane = threadIdx.x % WAVE;
     bool later[2] = {false, false};
     float more[2] = {0.f, 0.f};
-    const int n = min(a.k, WAVE), n2 = a.k - n;
-    for (int j = 0; j < n; ++j) {
-      const int c = __builtin_amdgcn_readlane(column[0], j);
-      const float qj = __uint_as_float(
-          __builtin_amdgcn_readlane(__float_as_uint(q[0]), j));
-      if (column[0] == c && j != lane) {
-        later[0] |= j < lane;
-        more[0] += qj;
-      }
-      if (column[1] == c) later[1] = true;
-    }
-    for (int j = 0; j < n2; ++j) {
-      const int c = __builtin_amdgcn_readlane(column[1], j);
-      const float qj = __uint_as_float(
-          __builtin_amdgcn_readlane(__float_as_uint(q[1]), j));
-      if (column[0] == c) more[0] += qj;
-      if (column[1] == c && j != lane) {
-        later[1] |= j < lane;
-        more[1] += qj;
+    for (int j = 0; j < a.k; ++j) {
+      const int h = j / WAVE;
+      const int c = __builtin_amdgcn_readlane(h ? column[1] : column[0], j % WAVE);
+      const float qj = __uint_as_float(__builtin_amdgcn_readlane(
+          __float_as_uint(h ? q[1] : q[0]), j % WAVE));
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (column[g] != c || lane + g * WAVE == j) continue;
+        later[g] |= j < lane + g * WAVE;
+        more[g] += qj;
       }
     }
 #pragma unroll
@@ -685,14 +712,6 @@ struct Teacher {
       }
       if (later[h]) column[h] = -1;
     }
-    hard = a.labels != nullptr && a.weight != 1.f;
-    y = -1;
-    zy = nan_value();
-    if (hard && label >= 0 && label < a.classes) {
-      y = (int)label;
-      zy = E::widen(z_row[label]);
-    }
-    seen = __ballot(y >= 0 && (column[0] == y || column[1] == y)) != 0;
   }
 
   // the row's loss; all lanes of the first wave
@@ -826,7 +845,7 @@ __device__ __forceinline__ void write_zeros(typename E::Raw* g, int first,
 // registers, kLoads 16-byte loads a thread: the logits are read once.
 template <typename E, int kThreads, int kLoads>
 __global__ void __launch_bounds__(kThreads)
-    distill_fused_kernel(Distill a) {
+    __attribute__((amdgpu_waves_per_eu(4))) distill_fused_kernel(Distill a) {
   constexpr int kV = E::kVec, kWaves = kThreads / WAVE;
   __shared__ float lds_max[kWaves];
   __shared__ Sums lds_sums[kWaves];
@@ -849,7 +868,8 @@ __global__ void __launch_bounds__(kThreads)
   const int wave = threadIdx.x / WAVE;
   Teacher teacher;
   if (wave == 0) {
-    teacher.read<E>(a, row, z, label);
+    teacher.fetch(a, row);
+    teacher.read<E>(a, z, label);
     const float scale = inverse_count(a);
     if (threadIdx.x == 0) {
       lds_scale = scale;
@@ -869,9 +889,11 @@ __global__ void __launch_bounds__(kThreads)
   const float o = origin(m);
   Sums st = {m, 0.f, 0.f};
 #pragma unroll
-  for (int r = 0; r < kLoads; ++r)
+  for (int r = 0; r < kLoads; ++r) {
+    forget(v[r]);
     if (r * kThreads * kV < a.classes)
       add_exps<E>(v[r], o, a.inv_tau, a.mode, st);
+  }
   st.s = wave_sum(st.s);
   st.t = wave_sum(st.t);
   if (threadIdx.x % WAVE == 0) lds_sums[wave] = st;
@@ -907,16 +929,18 @@ __global__ void __launch_bounds__(kThreads)
   const float pt = (a.weight == 0.f ? 0.f : ct * q_sum) / st.t + wrong;
   const float p1 = c1 / st.s;
 #pragma unroll
-  for (int r = 0; r < kLoads; ++r)
+  for (int r = 0; r < kLoads; ++r) {
+    forget(v[r]);
     write_grad<E>(v[r], o, a.inv_tau, a.mode, pt, p1, g,
                   (r * kThreads + (int)threadIdx.x) * kV, a.classes);
+  }
   __syncthreads();
   if (wave == 0) teacher.patch<E>(a, st, pt, p1, ct, c1, g, 0, a.classes);
 }
 
 constexpr int kSweep = 256;
 
-// The sums of a part of a row.
+// The sums of a part of a row, and of a whole one the loss.
 template <typename E>
 __global__ void __launch_bounds__(kSweep) distill_sums_kernel(Distill a) {
   constexpr int kV = E::kVec;
@@ -925,7 +949,11 @@ __global__ void __launch_bounds__(kSweep) distill_sums_kernel(Distill a) {
   const int64_t row = grid_row(a.splits);
   if (row >= a.rows) return;
   const int part = blockIdx.x % a.splits;
-  if (a.labels && a.labels[row] == a.ignore) return;
+  const int64_t label = a.labels ? a.labels[row] : 0;
+  if (a.labels && label == a.ignore) {
+    if (a.splits == 1 && threadIdx.x == 0) a.row_loss[row] = 0.f;
+    return;
+  }
   const typename E::Raw* z =
       (const typename E::Raw*)a.logits + row * a.row_stride;
   const int first = part * a.part_size;
@@ -963,6 +991,13 @@ __global__ void __launch_bounds__(kSweep) distill_sums_kernel(Distill a) {
     p[1] = st.s;
     p[2] = st.t;
   }
+  if (a.splits == 1 && threadIdx.x < WAVE) {
+    Teacher teacher;
+    teacher.fetch(a, row);
+    teacher.read<E>(a, z, label);
+    const float loss = teacher.loss(a, st);
+    if (threadIdx.x == 0) a.row_loss[row] = loss;
+  }
 }
 
 __device__ __forceinline__ Sums row_sums(const Distill& a, int64_t row) {
@@ -975,7 +1010,7 @@ __device__ __forceinline__ Sums row_sums(const Distill& a, int64_t row) {
   return wave_join(st, a.inv_tau);
 }
 
-// The rows' losses from their sums: one wave a row.
+// The split rows' losses from their sums: one wave a row.
 template <typename E>
 __global__ void __launch_bounds__(WAVE) distill_loss_kernel(Distill a) {
   const int64_t row = grid_row(1);
@@ -984,8 +1019,8 @@ __global__ void __launch_bounds__(WAVE) distill_loss_kernel(Distill a) {
   float loss = 0.f;
   if (!(a.labels && label == a.ignore)) {
     Teacher teacher;
-    teacher.read<E>(a, row,
-                    (const typename E::Raw*)a.logits + row * a.row_stride,
+    teacher.fetch(a, row);
+    teacher.read<E>(a, (const typename E::Raw*)a.logits + row * a.row_stride,
                     label);
     loss = teacher.loss(a, row_sums(a, row));
   }
@@ -1020,7 +1055,8 @@ __global__ void __launch_bounds__(kSweep) distill_grad_kernel(Distill a) {
   const int wave = threadIdx.x / WAVE;
   Teacher teacher;
   if (wave == 0) {
-    teacher.read<E>(a, row, z, label);
+    teacher.fetch(a, row);
+    teacher.read<E>(a, z, label);
     const float scale = inverse_count(a) * a.up[a.up_per_row ? row : 0];
     if (threadIdx.x == 0) {
       lds_scale = scale;
@@ -1087,7 +1123,7 @@ __global__ void __launch_bounds__(1024)
 
 // A row is split where there are too few rows to fill the card: into parts
 // of one chunk of a 256-thread workgroup at least.
-constexpr int kFill = 1024;  // workgroups: four for each of 256 CUs
+constexpr int kFill = 512;  // workgroups: two for each of 256 CUs
 
 int splits_of(int64_t rows, int classes, int vec, int* part) {
   if (rows < 1) rows = 1;
@@ -1148,6 +1184,7 @@ template <typename E>
 void distill_loss(const Distill& a, hipStream_t stream) {
   hipLaunchKernelGGL((distill_sums_kernel<E>), grid_of(a.rows, a.splits),
                      dim3(kSweep), 0, stream, a);
+  if (a.splits == 1) return;
   hipLaunchKernelGGL((distill_loss_kernel<E>), grid_of(a.rows, 1), dim3(WAVE), 0,
                      stream, a);
 }
