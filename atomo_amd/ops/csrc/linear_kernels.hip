@@ -161,6 +161,36 @@ __device__ __forceinline__ int slot(int row, int c) {
   return row * kRowChunks + (c ^ ((row ^ (row >> 3)) & 7));
 }
 
+// A row of a bf16 plane of an fp32 tile: 32 elements, four chunks.  Eight
+// neighbouring rows, and sixteen, fall on different banks.
+constexpr int kThirdBytes = 64;
+__device__ __forceinline__ int third_slot(int row, int c) {
+  return row * 4 + (c ^ ((row >> 1) & 3) ^ ((row >> 3) & 3));
+}
+
+// Elements 4 c4 .. 4 c4 + 3 of a row as x = a + b + c: a the bf16 next to x, b
+// the one next to x - a, c the rest: 3 x 8 bits hold the 24 of an fp32.
+__device__ __forceinline__ void put_thirds(char* tile, int plane, int row, int c4,
+                                           const u32x4& x) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  char* to = tile + third_slot(row, c4 / 2) * 16 + c4 % 2 * 8;
+  float r[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = __uint_as_float(x[e]);
+#pragma unroll
+  for (int t = 0; t < 3; ++t) {
+    u32x2 out;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bf16x2 near = {(__bf16)r[2 * h], (__bf16)r[2 * h + 1]};
+      out[h] = __builtin_bit_cast(uint32_t, near);
+      r[2 * h] -= __uint_as_float(out[h] << 16);
+      r[2 * h + 1] -= __uint_as_float(out[h] & 0xFFFF0000u);
+    }
+    *(u32x2*)(to + t * plane) = out;
+  }
+}
+
 // Tile of kRows rows by kRowBytes of the reduction, from memory to LDS.  What
 // is loaded is not touched before store(), so that nothing waits for it.
 template <typename E, int kRows, int kThreads, bool kAcross>
@@ -335,6 +365,29 @@ struct Stage {
     }
   }
 
+  // fp32 as three bf16 planes, `plane` bytes apart
+  __device__ __forceinline__ void store_thirds(char* tile, int plane) const {
+    static_assert(kC == 4, "fp32");
+    if constexpr (!kAcross) {
+#pragma unroll
+      for (int s = 0; s < kVecs; ++s) {
+        const int id = threadIdx.x + s * kThreads;
+        put_thirds(tile, plane, id / kRowChunks, id % kRowChunks, v[s]);
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const int id = threadIdx.x + b * kThreads;
+        if (idle(id)) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          put_thirds(tile, plane, id % (kRows / 4) * 4 + i, id / (kRows / 4),
+                     u32x4{v[b * 4][i], v[b * 4 + 1][i], v[b * 4 + 2][i],
+                           v[b * 4 + 3][i]});
+      }
+    }
+  }
+
   __device__ __forceinline__ void store(u32x4* tile) const {
     if constexpr (!kAcross) {
 #pragma unroll
@@ -440,6 +493,115 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// Which part of a product a workgroup makes.
+template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ>
+struct Work {
+  using Raw = typename E::Raw;
+  static constexpr int kK = kRowBytes / sizeof(Raw);  // a step's reduction
+  int part, i0, j0, rows_i, rows_j, ks, steps, whole, begin;
+  const Raw *p, *q;
+
+  __device__ explicit Work(const AtomoProduct& a) {
+    // Workgroups go round the 8 XCDs: each is given neighbouring tiles, in
+    // bands of kBand, so that its L2 holds what they share (8192 x 4096 x 4096
+    // bf16: 398 -> 375 us).
+    constexpr int kXcds = 8, kBand = 4;
+    const int tiles_i = (a.ni + kI - 1) / kI, tiles_j = (a.nj + kJ - 1) / kJ;
+    const int tiles = tiles_i * tiles_j, all = tiles * a.splits;
+    const int xcd = blockIdx.x % kXcds;
+    const int at = xcd * (all / kXcds) + min(xcd, all % kXcds) +
+                   (int)(blockIdx.x / kXcds);
+    const int tile = at % tiles;
+    const int band = tile / (kBand * tiles_i), in = tile % (kBand * tiles_i);
+    const int band_j = min(kBand, tiles_j - band * kBand);
+    const int tile_i = in / band_j, tile_j = band * kBand + in % band_j;
+    part = at / tiles;
+    i0 = tile_i * kI;
+    j0 = tile_j * kJ;
+    rows_i = min(a.ni - i0, kI);
+    rows_j = min(a.nj - j0, kJ);
+    const int k0 = part * a.k_part;
+    ks = min(a.nk - k0, a.k_part);
+    steps = (ks + kK - 1) / kK;
+    p = (const Raw*)a.p + (kAcrossP ? (int64_t)k0 * a.ldp + i0 : i0 * a.ldp + k0);
+    q = (const Raw*)a.q + (kAcrossQ ? (int64_t)k0 * a.ldq + j0 : j0 * a.ldq + k0);
+    // steps that load_whole() may take
+    whole = (kAcrossP && rows_i % 4) || (kAcrossQ && rows_j % 4) ? 0 : ks / kK;
+    // Neighbours start at different steps: rows of a power of two bytes put
+    // all that one step reads on a few of L2's channels (dW of 8192 x 4096 x
+    // 4096 bf16: 619 -> 322 us).  The order of the sum depends on the tile
+    // alone.
+    begin = (tile_i + tile_j) % 16 * 2 % steps;
+  }
+
+  template <bool kTiny, typename P, typename Q>
+  __device__ __forceinline__ void load(const AtomoProduct& a, int s, P& sp,
+                                       Q& sq) const {
+    s += begin;
+    s = s < steps ? s : s - steps;
+    const Raw* at_p = p + s * (kAcrossP ? a.ldp * kK : (int64_t)kK);
+    const Raw* at_q = q + s * (kAcrossQ ? a.ldq * kK : (int64_t)kK);
+    if constexpr (kTiny) {
+      sp.load_tiny(at_p, a.ldp, rows_i, ks - s * kK);
+      sq.load_tiny(at_q, a.ldq, rows_j, ks - s * kK);
+    } else if (s < whole) {
+      sp.load_whole(at_p, a.ldp, rows_i);
+      sq.load_whole(at_q, a.ldq, rows_j);
+    } else {
+      sp.load_edge(at_p, a.ldp, rows_i, ks - s * kK);
+      sq.load_edge(at_q, a.ldq, rows_j, ks - s * kK);
+    }
+  }
+};
+
+// A wave's sums, from row i0 and column j0 of the result on, to the epilogue
+// or to `partial`.  A lane holds i = 8 g + 4 (lane / 32) + 0..3 of j =
+// lane % 32.  By way of LDS (`mine`, the wave's own part, rows padded by 16
+// bytes against the banks) it gets four neighbours of a row of kPass, so that
+// lines are written whole and the epilogue's code is a short loop.
+template <int kFi>
+constexpr int pass_floats() {
+  return 32 * ((kFi > 1 ? 64 : 32) + 4);
+}
+
+template <typename E, int kFi, int kFj>
+__device__ __forceinline__ void write_tile(const AtomoProduct& a, int part,
+                                           int i0, int64_t j0,
+                                           const f32x16 (&acc)[kFi][kFj],
+                                           float* mine) {
+  constexpr int kPass = kFi > 1 ? 64 : 32, kPitch = kPass + 4;
+  constexpr int kLanes = kPass / 4;  // of a row
+  const int lane = threadIdx.x % 64;
+#pragma unroll
+  for (int ti = 0; ti < kFi; ti += kPass / 32)
+#pragma unroll
+    for (int tj = 0; tj < kFj; ++tj) {
+#pragma unroll
+      for (int t = 0; t < kPass / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(float4*)(mine + lane % 32 * kPitch + t * 32 + g * 8 + lane / 32 * 4) =
+              make_float4(acc[ti + t][tj][g * 4], acc[ti + t][tj][g * 4 + 1],
+                          acc[ti + t][tj][g * 4 + 2], acc[ti + t][tj][g * 4 + 3]);
+      wave_sync();
+#pragma unroll 1
+      for (int r = lane / kLanes; r < 32; r += 64 / kLanes) {
+        const float4 v = *(const float4*)(mine + r * kPitch + lane % kLanes * 4);
+        const int64_t j = j0 + tj * 32 + r;
+        const int i = i0 + ti * 32 + lane % kLanes * 4;
+        if (j >= a.nj || i >= a.ni) continue;
+        if (a.splits == 1) {
+          const float sum[4] = {v.x, v.y, v.z, v.w};
+          finish<E>(a, j, i, sum);
+        } else {
+          // rows of a multiple of four: whole vectors
+          *(float4*)(a.partial + ((int64_t)part * a.nj + j) * a.ld_part + i) = v;
+        }
+      }
+      wave_sync();
+    }
+}
+
 // kI x kJ of the result by kWi x kWj waves; a tile of the reduction is 128
 // bytes of each row, double-buffered in LDS.  With several parts of the
 // reduction (`splits`) each leaves its fp32 sums for join_parts_kernel.
@@ -447,71 +609,24 @@ template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
           int kWj, bool kTiny>
 __global__ void __launch_bounds__(kWi* kWj * 64)
     product_kernel(AtomoProduct a) {
-  using Raw = typename E::Raw;
   constexpr int kThreads = kWi * kWj * 64;
-  constexpr int kK = kRowBytes / sizeof(Raw);
   constexpr int kFi = kI / kWi / 32, kFj = kJ / kWj / 32;
   __shared__ u32x4 lds[2][(kI + kJ) * kRowChunks];
+  static_assert(kWi * kWj * pass_floats<kFi>() * 4 <= (int)sizeof(lds), "LDS");
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  // Workgroups go round the 8 XCDs: each is given neighbouring tiles, in bands
-  // of kBand, so that its L2 holds what they share (8192 x 4096 x 4096 bf16:
-  // 398 -> 375 us).
-  constexpr int kXcds = 8, kBand = 4;
-  const int tiles_i = (a.ni + kI - 1) / kI, tiles_j = (a.nj + kJ - 1) / kJ;
-  const int tiles = tiles_i * tiles_j, all = tiles * a.splits;
-  const int xcd = blockIdx.x % kXcds;
-  const int at = xcd * (all / kXcds) + min(xcd, all % kXcds) +
-                 (int)(blockIdx.x / kXcds);
-  const int part = at / tiles, tile = at % tiles;
-  const int band = tile / (kBand * tiles_i), in_band = tile % (kBand * tiles_i);
-  const int band_j = min(kBand, tiles_j - band * kBand);
-  const int tile_i = in_band / band_j, tile_j = band * kBand + in_band % band_j;
-  const int i0 = tile_i * kI, j0 = tile_j * kJ;
-  const int rows_i = min(a.ni - i0, kI), rows_j = min(a.nj - j0, kJ);
-  const int k0 = part * a.k_part, ks = min(a.nk - k0, a.k_part);
-  const Raw* p = (const Raw*)a.p +
-                 (kAcrossP ? (int64_t)k0 * a.ldp + i0 : i0 * a.ldp + k0);
-  const Raw* q = (const Raw*)a.q +
-                 (kAcrossQ ? (int64_t)k0 * a.ldq + j0 : j0 * a.ldq + k0);
-  const int64_t step_p = kAcrossP ? a.ldp * kK : kK;
-  const int64_t step_q = kAcrossQ ? a.ldq * kK : kK;
-  const int steps = (ks + kK - 1) / kK;
-
-  // steps that load_whole() may take
-  const int whole = (kAcrossP && rows_i % 4) || (kAcrossQ && rows_j % 4)
-                        ? 0
-                        : ks / kK;
-
-  // Neighbours start at different steps: rows of a power of two bytes put all
-  // that one step reads on a few of L2's channels (dW of 8192 x 4096 x 4096
-  // bf16: 619 -> 322 us).  The order of the sum depends on the tile alone.
-  const int begin = (tile_i + tile_j) % 16 * 2 % steps;
+  const Work<E, kAcrossP, kAcrossQ, kI, kJ> work(a);
 
   f32x16 acc[kFi][kFj] = {};
   Stage<E, kI, kThreads, kAcrossP> sp;
   Stage<E, kJ, kThreads, kAcrossQ> sq;
-  const auto load = [&](int s) {
-    s += begin;
-    s = s < steps ? s : s - steps;
-    if constexpr (kTiny) {
-      sp.load_tiny(p + s * step_p, a.ldp, rows_i, ks - s * kK);
-      sq.load_tiny(q + s * step_q, a.ldq, rows_j, ks - s * kK);
-    } else if (s < whole) {
-      sp.load_whole(p + s * step_p, a.ldp, rows_i);
-      sq.load_whole(q + s * step_q, a.ldq, rows_j);
-    } else {
-      sp.load_edge(p + s * step_p, a.ldp, rows_i, ks - s * kK);
-      sq.load_edge(q + s * step_q, a.ldq, rows_j, ks - s * kK);
-    }
-  };
-  load(0);
+  work.template load<kTiny>(a, 0, sp, sq);
   sp.store(lds[0]);
   sq.store(lds[0] + kI * kRowChunks);
   __syncthreads();
   const int wi = wave % kWi * (kI / kWi), wj = wave / kWi * (kJ / kWj);
-  for (int s = 0; s < steps; ++s) {
-    const bool more = s + 1 < steps;
-    if (more) load(s + 1);
+  for (int s = 0; s < work.steps; ++s) {
+    const bool more = s + 1 < work.steps;
+    if (more) work.template load<kTiny>(a, s + 1, sp, sq);
     const u32x4* tp = lds[s & 1];
     const u32x4* tq = tp + kI * kRowChunks;
 #pragma unroll
@@ -532,43 +647,101 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
     }
     __syncthreads();
   }
+  write_tile<E>(a, work.part, work.i0 + wi, work.j0 + wj, acc,
+                (float*)lds + wave * pass_floats<kFi>());
+}
 
-  // A lane holds i = 8 g + 4 (lane / 32) + 0..3 of j = lane % 32.  By way of
-  // LDS (each wave its own part, rows padded by 16 bytes against the banks) it
-  // gets four neighbours of a row of kPass, so that lines are written whole
-  // and the epilogue's code is a short loop.
-  constexpr int kPass = kFi > 1 ? 64 : 32, kPitch = kPass + 4;
-  constexpr int kLanes = kPass / 4;  // of a row
-  static_assert(kWi * kWj * 32 * kPitch * 4 <= (int)sizeof(lds), "fits LDS");
-  float* mine = (float*)lds + wave * 32 * kPitch;
+// The same for fp32 operands on the bf16 matrix instructions, 16 times as fast
+// as the fp32 ones: with x = a + b + c and y = a' + b' + c' (put_thirds) the
+// six products aa', ab', ba', bb', ac', ca' are xy but for 2^-25 of it, less
+// than fp32 loses by its sums.  2.7 times less time in matrix instructions
+// (128 x 9216 x 4096, forward / dx / dW: 100 / 109 / 139 us by fp32
+// instructions).  One buffer in LDS, so that three workgroups share a CU and
+// fill each other's waits.
+//
+// Where a sum comes out infinite or NaN (0 times a split infinity is NaN, and
+// so is what rounds up to one) the tile is made again, by fp32 instructions.
+template <bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi, int kWj>
+__global__ void __launch_bounds__(kWi* kWj * 64)
+    product_thirds_kernel(AtomoProduct a) {
+  constexpr int kThreads = kWi * kWj * 64;
+  constexpr int kFi = kI / kWi / 32, kFj = kJ / kWj / 32;
+  constexpr int kPlane = (kI + kJ) * kThirdBytes;
+  __shared__ u32x4 lds[3 * kPlane / 16];
+  static_assert(kWi * kWj * pass_floats<kFi>() * 4 <= (int)sizeof(lds), "LDS");
+  char* tile_p = (char*)lds;
+  char* tile_q = tile_p + kI * kThirdBytes;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const Work<F32, kAcrossP, kAcrossQ, kI, kJ> work(a);
+
+  f32x16 acc[kFi][kFj] = {};
+  Stage<F32, kI, kThreads, kAcrossP> sp;
+  Stage<F32, kJ, kThreads, kAcrossQ> sq;
+  work.template load<false>(a, 0, sp, sq);
+  const int wi = wave % kWi * (kI / kWi), wj = wave / kWi * (kJ / kWj);
+  for (int s = 0; s < work.steps; ++s) {
+    sp.store_thirds(tile_p, kPlane);
+    sq.store_thirds(tile_q, kPlane);
+    __syncthreads();
+    if (s + 1 < work.steps) work.template load<false>(a, s + 1, sp, sq);
 #pragma unroll
-  for (int ti = 0; ti < kFi; ti += kPass / 32)
+    for (int c = 0; c < 4; c += 2) {
+      u32x4 fp[3][kFi], fq[3][kFj];
 #pragma unroll
-    for (int tj = 0; tj < kFj; ++tj) {
+      for (int h = 0; h < 3; ++h) {
 #pragma unroll
-      for (int t = 0; t < kPass / 32; ++t)
+        for (int t = 0; t < kFi; ++t)
+          fp[h][t] = *(const u32x4*)(tile_p + h * kPlane +
+                                     third_slot(wi + t * 32 + lane % 32,
+                                                c + lane / 32) * 16);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *(float4*)(mine + lane % 32 * kPitch + t * 32 + g * 8 + lane / 32 * 4) =
-              make_float4(acc[ti + t][tj][g * 4], acc[ti + t][tj][g * 4 + 1],
-                          acc[ti + t][tj][g * 4 + 2], acc[ti + t][tj][g * 4 + 3]);
-      wave_sync();
-#pragma unroll 1
-      for (int r = lane / kLanes; r < 32; r += 64 / kLanes) {
-        const float4 v = *(const float4*)(mine + r * kPitch + lane % kLanes * 4);
-        const int64_t j = j0 + wj + tj * 32 + r;
-        const int i = i0 + wi + ti * 32 + lane % kLanes * 4;
-        if (j >= a.nj || i >= a.ni) continue;
-        if (a.splits == 1) {
-          const float sum[4] = {v.x, v.y, v.z, v.w};
-          finish<E>(a, j, i, sum);
-        } else {
-          // rows of a multiple of four: whole vectors
-          *(float4*)(a.partial + ((int64_t)part * a.nj + j) * a.ld_part + i) = v;
+        for (int t = 0; t < kFj; ++t)
+          fq[h][t] = *(const u32x4*)(tile_q + h * kPlane +
+                                     third_slot(wj + t * 32 + lane % 32,
+                                                c + lane / 32) * 16);
+      }
+      // the small ones first
+      multiply<BF16>(fp[2], fq[0], acc);
+      multiply<BF16>(fp[0], fq[2], acc);
+      multiply<BF16>(fp[1], fq[1], acc);
+      multiply<BF16>(fp[1], fq[0], acc);
+      multiply<BF16>(fp[0], fq[1], acc);
+      multiply<BF16>(fp[0], fq[0], acc);
+    }
+    __syncthreads();
+  }
+  float odd = 0.f;  // NaN where a sum is not finite
+#pragma unroll
+  for (int ti = 0; ti < kFi; ++ti)
+#pragma unroll
+    for (int tj = 0; tj < kFj; ++tj)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) odd += acc[ti][tj][e] * 0.f;
+  if (__ballot(odd != odd) != 0) {
+    // 32 x 32 after 32 x 32: rare, so short rather than fast
+#pragma unroll
+    for (int ti = 0; ti < kFi; ++ti)
+#pragma unroll
+      for (int tj = 0; tj < kFj; ++tj) {
+        const int64_t i = min(wi + ti * 32 + lane % 32, work.rows_i - 1);
+        const int64_t j = min(wj + tj * 32 + lane % 32, work.rows_j - 1);
+        const uint32_t* x = work.p + (kAcrossP ? i : i * a.ldp);
+        const uint32_t* y = work.q + (kAcrossQ ? j : j * a.ldq);
+        acc[ti][tj] = f32x16{};
+        // lane halves take neighbouring k
+        for (int k = 0; k < work.ks; k += 2) {
+          const int64_t at = min(k + lane / 32, work.ks - 1);
+          float u = __uint_as_float(x[kAcrossP ? at * a.ldp : at]);
+          float v = __uint_as_float(y[kAcrossQ ? at * a.ldq : at]);
+          u = k + lane / 32 < work.ks ? u : 0.f;
+          v = k + lane / 32 < work.ks ? v : 0.f;
+          acc[ti][tj] = __builtin_amdgcn_mfma_f32_32x32x2f32(u, v, acc[ti][tj],
+                                                             0, 0, 0);
         }
       }
-      wave_sync();
-    }
+  }
+  write_tile<F32>(a, work.part, work.i0 + wi, work.j0 + wj, acc,
+                  (float*)lds + wave * pass_floats<kFi>());
 }
 
 constexpr int kThreads = 256;
@@ -802,19 +975,27 @@ __global__ void __launch_bounds__(kDpWaves * 64)
   }
 }
 
-template <typename E, int kI, int kJ, int kWi, int kWj, bool kTiny = false>
-void product(const AtomoProduct& a, hipStream_t stream) {
+template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
+          int kWj, bool kTiny>
+void launch_product(const AtomoProduct& a, hipStream_t stream) {
   const int64_t tiles = (int64_t)((a.ni + kI - 1) / kI) * ((a.nj + kJ - 1) / kJ);
   const dim3 grid((unsigned)(tiles * a.splits)), block(kWi * kWj * 64);
-  if (a.form == ATOMO_FORWARD)
-    hipLaunchKernelGGL((product_kernel<E, false, false, kI, kJ, kWi, kWj, kTiny>),
-                       grid, block, 0, stream, a);
-  else if (a.form == ATOMO_GRAD_X)
-    hipLaunchKernelGGL((product_kernel<E, true, false, kI, kJ, kWi, kWj, kTiny>),
+  if constexpr (E::kChunk == 4 && !kTiny)
+    hipLaunchKernelGGL((product_thirds_kernel<kAcrossP, kAcrossQ, kI, kJ, kWi, kWj>),
                        grid, block, 0, stream, a);
   else
-    hipLaunchKernelGGL((product_kernel<E, true, true, kI, kJ, kWi, kWj, kTiny>),
+    hipLaunchKernelGGL((product_kernel<E, kAcrossP, kAcrossQ, kI, kJ, kWi, kWj, kTiny>),
                        grid, block, 0, stream, a);
+}
+
+template <typename E, int kI, int kJ, int kWi, int kWj, bool kTiny = false>
+void product(const AtomoProduct& a, hipStream_t stream) {
+  if (a.form == ATOMO_FORWARD)
+    launch_product<E, false, false, kI, kJ, kWi, kWj, kTiny>(a, stream);
+  else if (a.form == ATOMO_GRAD_X)
+    launch_product<E, true, false, kI, kJ, kWi, kWj, kTiny>(a, stream);
+  else
+    launch_product<E, true, true, kI, kJ, kWi, kWj, kTiny>(a, stream);
 }
 
 template <typename E, int kM>

@@ -205,6 +205,33 @@ def test_infinite_inputs():
             assert y[1].isnan().all()
 
 
+@pytest.mark.parametrize("m,k,n", [(3, 20, 5), (130, 200, 140), (40, 3000, 70)])
+def test_single_infinities_and_extremes(m, k, n):
+    """An infinity times finite numbers, one by one: what fp32 gives, and
+    nothing next to it; operands at both ends of fp32."""
+    x, w = _grid((m, k), 1, F32) + 20, _grid((n, k), 2, F32) + 10.5  # no zeros
+    x[m // 2, k // 3], x[m - 1, k - 1] = math.inf, 3.4e38
+    x[0], w[0, 0] = x[0] * 2.0 ** -120, math.nan
+    cx, cw = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y = linear_ops.linear_act(cx, cw)
+    want = (x.double() @ w.double().t()).float()
+    got = y.detach().cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.isinf(), want.isinf())
+    ok = torch.isfinite(want)
+    # products of 2^-120 parts: their third parts lie below fp32's normal
+    # numbers, 2^-126, and may be taken for 0; else k half steps of the sums
+    tiny = k * 2.0 ** -126 * 32
+    size = x.abs().double() @ w.abs().double().t()
+    assert ((got.double() - want.double()).abs() <= (k + 2) * U * size + tiny)[ok].all()
+    gx, gw = torch.autograd.grad(y, (cx, cw), torch.ones_like(y))
+    want = (torch.ones(m, n).double() @ w.double()).float()
+    assert torch.equal(gx.cpu().isnan(), want.isnan())
+    want = (torch.ones(n, m).double() @ x.double()).float()
+    assert torch.equal(gw.cpu().isinf(), want.isinf())
+    assert not gw.isnan().any()
+
+
 @pytest.mark.parametrize("m,k,n,dtype", [(1, 500, 300, BF16), (128, 784, 800, F32), (300, 300, 600, F16)])
 def test_in_a_graph(m, k, n, dtype):
     """Forward and backward captured together, replayed between eager passes
