@@ -40,7 +40,9 @@ struct AtomoProduct {
   int64_t ldp, ldq, ldo, ldr, ld_part;
   int ni, nj, nk;
   int type, form, act;
-  int plan, splits, k_part;  // by atomo_product_plan
+  // by atomo_product_plan, from all above but `partial`; `bare`: the tiles
+  // have no epilogue
+  int plan, splits, k_part, bare;
 };
 
 // dp = dy * slope, where dp is wanted; db, the sums of its columns, likewise.

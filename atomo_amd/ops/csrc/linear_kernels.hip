@@ -554,6 +554,29 @@ struct Work {
   }
 };
 
+// Four neighbouring sums without an epilogue, or of a part of the reduction.
+template <typename E>
+__device__ __forceinline__ void put_bare(const AtomoProduct& a, int part,
+                                         int64_t j, int i, const float4& v) {
+  using Raw = typename E::Raw;
+  if (i >= a.ni) return;
+  if (a.splits > 1) {
+    // rows of a multiple of four: whole vectors
+    *(float4*)(a.partial + ((int64_t)part * a.nj + j) * a.ld_part + i) = v;
+    return;
+  }
+  const Four<Raw> y = {{E::narrow(v.x), E::narrow(v.y), E::narrow(v.z),
+                        E::narrow(v.w)}};
+  Raw* out = (Raw*)a.out + j * a.ldo + i;
+  if (i + 4 <= a.ni) {
+    *(Four<Raw>*)out = y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (i + e < a.ni) out[e] = y.v[e];
+  }
+}
+
 // A wave's sums, from row i0 and column j0 of the result on, to the epilogue
 // or to `partial`.  A lane holds i = 8 g + 4 (lane / 32) + 0..3 of j =
 // lane % 32.  By way of LDS (`mine`, the wave's own part, rows padded by 16
@@ -584,18 +607,25 @@ __device__ __forceinline__ void write_tile(const AtomoProduct& a, int part,
               make_float4(acc[ti + t][tj][g * 4], acc[ti + t][tj][g * 4 + 1],
                           acc[ti + t][tj][g * 4 + 2], acc[ti + t][tj][g * 4 + 3]);
       wave_sync();
+      constexpr int kRows = 64 / kLanes;  // of the pass, at a time
+      const int i = i0 + ti * 32 + lane % kLanes * 4;
+      const int64_t j = j0 + tj * 32 + lane / kLanes;
+      const float* from = mine + lane / kLanes * kPitch + lane % kLanes * 4;
+      if (a.bare) {
+        // nothing but stores: all reads go before the first
+        float4 v[32 / kRows];
+#pragma unroll
+        for (int r = 0; r < 32 / kRows; ++r)
+          v[r] = *(const float4*)(from + r * kRows * kPitch);
+#pragma unroll
+        for (int r = 0; r < 32 / kRows; ++r)
+          if (j + r * kRows < a.nj) put_bare<E>(a, part, j + r * kRows, i, v[r]);
+      } else {
 #pragma unroll 1
-      for (int r = lane / kLanes; r < 32; r += 64 / kLanes) {
-        const float4 v = *(const float4*)(mine + r * kPitch + lane % kLanes * 4);
-        const int64_t j = j0 + tj * 32 + r;
-        const int i = i0 + ti * 32 + lane % kLanes * 4;
-        if (j >= a.nj || i >= a.ni) continue;
-        if (a.splits == 1) {
+        for (int r = 0; r < 32; r += kRows) {
+          const float4 v = *(const float4*)(from + r * kPitch);
           const float sum[4] = {v.x, v.y, v.z, v.w};
-          finish<E>(a, j, i, sum);
-        } else {
-          // rows of a multiple of four: whole vectors
-          *(float4*)(a.partial + ((int64_t)part * a.nj + j) * a.ld_part + i) = v;
+          if (j + r < a.nj) finish<E>(a, j + r, i, sum);
         }
       }
       wave_sync();
@@ -663,7 +693,7 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
 // so is what rounds up to one) the tile is made again, by fp32 instructions.
 template <bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi, int kWj>
 __global__ void __launch_bounds__(kWi* kWj * 64)
-    product_thirds_kernel(AtomoProduct a) {
+    __attribute__((amdgpu_waves_per_eu(3))) product_thirds_kernel(AtomoProduct a) {
   constexpr int kThreads = kWi * kWj * 64;
   constexpr int kFi = kI / kWi / 32, kFj = kJ / kWj / 32;
   constexpr int kPlane = (kI + kJ) * kThirdBytes;
@@ -1104,6 +1134,8 @@ void atomo_product_plan(AtomoProduct* a) {
     a->splits = (steps + part - 1) / part;
   }
   a->ld_part = (a->ni + 3) / 4 * 4;
+  a->bare = a->splits > 1 || (a->act == ATOMO_ACT_NONE && !a->bias &&
+                              !a->residual && !a->slope);
 }
 
 void atomo_product_launch(const AtomoProduct* a, hipStream_t stream) {
