@@ -652,11 +652,10 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
   work.template load<kTiny>(a, 0, sp, sq);
   sp.store(lds[0]);
   sq.store(lds[0] + kI * kRowChunks);
+  if (work.steps > 1) work.template load<kTiny>(a, 1, sp, sq);
   __syncthreads();
   const int wi = wave % kWi * (kI / kWi), wj = wave / kWi * (kJ / kWj);
   for (int s = 0; s < work.steps; ++s) {
-    const bool more = s + 1 < work.steps;
-    if (more) work.template load<kTiny>(a, s + 1, sp, sq);
     const u32x4* tp = lds[s & 1];
     const u32x4* tq = tp + kI * kRowChunks;
 #pragma unroll
@@ -670,11 +669,15 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
         fq[t] = tq[slot(wj + t * 32 + lane % 32, c + lane / 32)];
       multiply<E>(fp, fq, acc);
     }
-    if (more) {
+    // the next step's tile, loaded a step ago, while the matrix instructions
+    // drain (8192 x 4096 x 4096 bf16: 326 / 343 / 312 -> 314 / 301 / 296 us),
+    // and the loads of the one after it
+    if (s + 1 < work.steps) {
       u32x4* to = lds[(s + 1) & 1];
       sp.store(to);
       sq.store(to + kI * kRowChunks);
     }
+    if (s + 2 < work.steps) work.template load<kTiny>(a, s + 2, sp, sq);
     __syncthreads();
   }
   write_tile<E>(a, work.part, work.i0 + wi, work.j0 + wj, acc,
