@@ -391,8 +391,11 @@ __global__ void __launch_bounds__(kThreads)
   float best[kParts];
 #pragma unroll
   for (int u = 0; u < kParts; ++u) best[u] = -kInf;
-  // loads that hold a class: the others have no part in the bar
-  const int filled = min(kParts * WAVE * kWaves, (end - first + kV - 1) / kV);
+  // Is there a class for each of the first loads of all threads (but for the
+  // last part of some rows, always), or, in one wave, for k loads?  Loads
+  // without one count as -inf, below no class.
+  const bool enough = kWaves > 1 ? end - first >= kThreads * kV
+                                 : (end - first + kV - 1) / kV >= top;
 
   Stat st = Stat::none();
   u32x4 now[kParts], next[kParts];
@@ -438,10 +441,8 @@ __global__ void __launch_bounds__(kThreads)
     if (top == 0) continue;
     // each wave's share of k of the maxima: the least of the bars has k above
     uint32_t low = 0;
-    if (filled == kParts * WAVE * kWaves)
-      low = wave_bar(best, (top + kWaves - 1) / kWaves);
-    else if (kWaves == 1 && filled >= top)
-      low = wave_bar(best, top);
+    static_assert(ATOMO_LOGIT_TOP_MAX <= WAVE * 4, "a wave's share of k");
+    if (enough) low = wave_bar(best, (top + kWaves - 1) / kWaves);
     if (kWaves > 1) {
       __syncthreads();
       if (lane == 0) bars[wave] = low;
@@ -480,7 +481,7 @@ __global__ void __launch_bounds__(kThreads)
         n += __popcll(mask);
       }
     }
-    if (kWaves > 1) __syncthreads();  // `tops` and `bars` are written again
+    if (kWaves > 1) __syncthreads();  // `bars` is written again
   }
 
   st = block_join<kThreads>(st, stats);
@@ -488,28 +489,9 @@ __global__ void __launch_bounds__(kThreads)
   if (top > 0) {
     if (lane == 0) counts[wave] = n;
     __syncthreads();
+    // A key's rank is the number of greater ones: of n candidates, mostly a
+    // little over k, n^2 / 256 reads for each thread.
     int all = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) all += counts[w];
-    if (all > kListSize) {
-      // into one list, filled no faster than it is read, and cut
-      if (wave == 0) {
-        int kept = counts[0];
-        for (int w = 1; w < kWaves; ++w) {
-          const int have = counts[w];
-          for (int i = lane; i < ((have + WAVE - 1) & -WAVE); i += WAVE) {
-            const uint64_t key = i < have ? lists[w * kListSize + i] : 0;
-            if (i < have) lists[kept + i] = key;
-          }
-          kept += have;
-        }
-        cut_list(lists, kept, top);
-        if (lane < kWaves) counts[lane] = lane == 0 ? top : 0;
-      }
-      __syncthreads();
-    }
-    // a key's rank is the number of greater ones
-    all = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) all += counts[w];
     for (int i = threadIdx.x; i < all; i += kThreads) {
@@ -1121,20 +1103,23 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// A row is split where there are too few rows to fill the card: into parts
-// of one chunk of a 256-thread workgroup at least.
+// A row is split where there are too few rows to fill the card, evenly, and so
+// that the parts are not much below a chunk of a 256-thread workgroup.
 constexpr int kFill = 512;  // workgroups: two for each of 256 CUs
 
 int splits_of(int64_t rows, int classes, int vec, int* part) {
   if (rows < 1) rows = 1;
-  const int chunk = 256 * kParts * vec;
+  const int64_t chunk = 256 * kParts * vec;
   int64_t n = (kFill + rows - 1) / rows;
   n = n < kMostSplits ? n : kMostSplits;
-  const int64_t chunks = (classes + (int64_t)chunk - 1) / chunk;
+  const int64_t chunks = (classes + chunk - 1) / chunk;
   n = n < chunks ? n : chunks;
-  if (n < 1) n = 1;
-  const int64_t size = (chunks + n - 1) / n * chunk;
-  *part = (int)(size < classes ? size : classes);
+  if (n <= 1) {
+    *part = classes;
+    return 1;
+  }
+  const int64_t size = ((classes + n - 1) / n + vec - 1) / vec * vec;
+  *part = (int)size;
   return (int)((classes + size - 1) / size);
 }
 

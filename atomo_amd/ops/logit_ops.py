@@ -122,8 +122,8 @@ def distill_loss(
     ``teacher_value`` (..., k) at the classes ``teacher_index`` (..., k), with
     ``weight``, and against ``labels`` (...) with ``1 - weight``.
 
-    The values may be logits or log probabilities: a constant added to a row
-    changes nothing.  k is at most 128; an entry of -inf is absent, and its
+    ``temperature`` lies in 0.01..100.  The values may be logits or log
+    probabilities: a constant added to a row changes nothing.  k is at most 128; an entry of -inf is absent, and its
     index is not looked at.  Any other index outside 0..classes-1 makes the
     row NaN, and so does such a label, except ``ignore_index``: that row has
     no loss, no gradient, and is not counted in the mean (of no rows: 0).
@@ -153,8 +153,9 @@ def distill_loss(
                       "teacher_index").view(-1, k)
     value = teacher_value.detach().float().contiguous().view(-1, k)
     temperature, weight = float(temperature), float(weight)
-    if not (math.isfinite(temperature) and temperature > 0.0):
-        raise ValueError(f"temperature must be positive, not {temperature}")
+    if not 0.01 <= temperature <= 100.0:
+        # tau^2 times what 32 bits lose of a distribution at tau
+        raise ValueError(f"temperature must lie in 0.01..100, not {temperature}")
     if not 0.0 <= weight <= 1.0:
         raise ValueError(f"weight must lie in 0..1, not {weight}")
     if labels is None and weight != 1.0:

@@ -99,6 +99,21 @@ class PSTrainer:
                 distill_from, distill_network or model_name, num_classes,
                 in_channels, fused_linear,
             )
+            from ..ops.logit_ops import TOP_MAX
+
+            if not 1 <= int(distill_top) <= TOP_MAX:
+                raise ValueError(
+                    f"--distill-top must lie in 1..{TOP_MAX}, not {distill_top}"
+                )
+            if not 0.0 <= float(distill_weight) <= 1.0:
+                raise ValueError(
+                    f"--distill-weight must lie in 0..1, not {distill_weight}"
+                )
+            if not 0.01 <= float(distill_temperature) <= 100.0:
+                raise ValueError(
+                    "--distill-temperature must lie in 0.01..100, not "
+                    f"{distill_temperature}"
+                )
             self.distill_top = min(int(distill_top), num_classes)
             self.distill_temperature = float(distill_temperature)
             self.distill_weight = float(distill_weight)

@@ -135,6 +135,15 @@ def test_logprobs_labels_outside_and_other_stream():
     assert none.top_index.shape == (0, 3)
 
 
+def test_more_rows_than_one_dimension_of_a_grid():
+    rows, classes = 300001, 3
+    z, cuda = _logits(rows, classes, F32)
+    y = _labels(rows, classes)
+    _check_logprobs(z, cuda, y, 2)
+    value, index = _teacher(1, classes, 2)
+    _check_distill(z, cuda, value.expand(rows, 2), index.expand(rows, 2).contiguous(), y, 2.0, 0.5)
+
+
 @pytest.mark.parametrize("rows,classes", [(1, 100000), (300, 10), (70, 5000)])
 def test_logprobs_in_a_graph(rows, classes):
     _, first = _logits(rows, classes, BF16, seed=1)

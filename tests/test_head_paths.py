@@ -143,6 +143,15 @@ def test_teacher_of_another_network_is_refused(tmp_path):
         _trainer(distill_from=path)
 
 
+@pytest.mark.parametrize("wrong", [
+    dict(distill_top=0), dict(distill_top=129), dict(distill_weight=1.5),
+    dict(distill_temperature=0.0)])
+def test_wrong_distillation_is_refused(tmp_path, wrong):
+    path = _trainer(train_dir=str(tmp_path)).save_checkpoint()
+    with pytest.raises(ValueError):
+        _trainer(distill_from=path, **wrong)
+
+
 def test_many_classes_keep_the_top():
     z = torch.randn(3, 300)
     assert label_logprobs(z, top=128).top_index.shape == (3, 128)

@@ -222,6 +222,7 @@ def test_distill_second_derivative_is_refused():
 
 
 @pytest.mark.parametrize("change,error", [
+    (dict(temperature=1e-3), ValueError), (dict(temperature=1e3), ValueError),
     (dict(temperature=0.0), ValueError), (dict(temperature=math.inf), ValueError),
     (dict(temperature=math.nan), ValueError), (dict(weight=1.5), ValueError),
     (dict(weight=math.nan), ValueError), (dict(weight=0.5, labels=None), ValueError),
