@@ -444,46 +444,62 @@ struct Four {
   Raw v[4];
 } __attribute__((packed, aligned(sizeof(Raw))));
 
-// bias, activation, residual and slope on four neighbouring sums of row j
+// the first n of four
+template <typename Raw>
+__device__ __forceinline__ Four<Raw> load_four(const Raw* at, int n) {
+  Four<Raw> f = {};
+  if (n >= 4) return *(const Four<Raw>*)at;
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < n) f.v[e] = at[e];
+  return f;
+}
+template <typename Raw>
+__device__ __forceinline__ void store_four(Raw* at, int n, const Four<Raw>& f) {
+  if (n >= 4) {
+    *(Four<Raw>*)at = f;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 3; ++e)
+    if (e < n) at[e] = f.v[e];
+}
+
+// Bias, activation, residual and slope on four neighbouring sums of row j, of
+// which the columns below a.ni exist.
 template <typename E>
 __device__ __forceinline__ void finish(const AtomoProduct& a, int64_t j, int i,
-                                       const float (&sum)[4]) {
+                                       const float (&sum)[4],
+                                       const Four<typename E::Raw>& bias,
+                                       const Four<typename E::Raw>& residual) {
   using Raw = typename E::Raw;
   using Slope = typename E::Slope;
-  const int n = min(4, a.ni - i);
-  if (n <= 0) return;
-  const Raw* bias = (const Raw*)a.bias;
-  const Raw* residual = (const Raw*)a.residual + j * a.ldr + i;
-  Slope* slope = (Slope*)a.slope + j * a.ni + i;
-  Raw* out = (Raw*)a.out + j * a.ldo + i;
-  Four<Raw> y, b, r;
+  Four<Raw> y;
   Four<Slope> s;
-  if (n == 4) {
-    if (a.bias) b = *(const Four<Raw>*)(bias + i);
-    if (a.residual) r = *(const Four<Raw>*)residual;
-  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (e >= n) break;
-    float h = sum[e];
-    if (a.bias) h += E::widen(n == 4 ? b.v[e] : bias[i + e]);
-    float d;
+    float h = sum[e], d;
+    if (a.bias) h += E::widen(bias.v[e]);
     h = activate<E::kChunk == 8>(a.act, h, &d);
     put_slope(&s.v[e], d);
-    if (a.residual) h += E::widen(n == 4 ? r.v[e] : residual[e]);
+    if (a.residual) h += E::widen(residual.v[e]);
     y.v[e] = E::narrow(h);
   }
-  if (n == 4) {
-    *(Four<Raw>*)out = y;
-    if (a.slope) *(Four<Slope>*)slope = s;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 3; ++e) {
-      if (e >= n) break;
-      out[e] = y.v[e];
-      if (a.slope) slope[e] = s.v[e];
-    }
-  }
+  store_four((Raw*)a.out + j * a.ldo + i, a.ni - i, y);
+  if (a.slope) store_four((Slope*)a.slope + j * a.ni + i, a.ni - i, s);
+}
+
+template <typename E>
+__device__ __forceinline__ Four<typename E::Raw> bias_of(const AtomoProduct& a,
+                                                         int i) {
+  if (!a.bias || i >= a.ni) return {};
+  return load_four((const typename E::Raw*)a.bias + i, a.ni - i);
+}
+template <typename E>
+__device__ __forceinline__ Four<typename E::Raw> residual_of(
+    const AtomoProduct& a, int64_t j, int i) {
+  if (!a.residual || i >= a.ni || j >= a.nj) return {};
+  return load_four((const typename E::Raw*)a.residual + j * a.ldr + i, a.ni - i);
 }
 
 // lanes of one wave read in LDS what others of it wrote
@@ -567,14 +583,7 @@ __device__ __forceinline__ void put_bare(const AtomoProduct& a, int part,
   }
   const Four<Raw> y = {{E::narrow(v.x), E::narrow(v.y), E::narrow(v.z),
                         E::narrow(v.w)}};
-  Raw* out = (Raw*)a.out + j * a.ldo + i;
-  if (i + 4 <= a.ni) {
-    *(Four<Raw>*)out = y;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (i + e < a.ni) out[e] = y.v[e];
-  }
+  store_four((Raw*)a.out + j * a.ldo + i, a.ni - i, y);
 }
 
 // A wave's sums, from row i0 and column j0 of the result on, to the epilogue
@@ -621,11 +630,25 @@ __device__ __forceinline__ void write_tile(const AtomoProduct& a, int part,
         for (int r = 0; r < 32 / kRows; ++r)
           if (j + r * kRows < a.nj) put_bare<E>(a, part, j + r * kRows, i, v[r]);
       } else {
+        // all that four rows need is read before the first is worked on
+        constexpr int kBatch = 32 / kRows < 4 ? 32 / kRows : 4;
+        const Four<typename E::Raw> bias = bias_of<E>(a, i);
 #pragma unroll 1
-        for (int r = 0; r < 32; r += kRows) {
-          const float4 v = *(const float4*)(from + r * kPitch);
-          const float sum[4] = {v.x, v.y, v.z, v.w};
-          if (j + r < a.nj) finish<E>(a, j + r, i, sum);
+        for (int r0 = 0; r0 < 32; r0 += kRows * kBatch) {
+          float4 v[kBatch];
+          Four<typename E::Raw> residual[kBatch];
+#pragma unroll
+          for (int r = 0; r < kBatch; ++r) {
+            residual[r] = residual_of<E>(a, j + r0 + r * kRows, i);
+            v[r] = *(const float4*)(from + (r0 + r * kRows) * kPitch);
+          }
+#pragma unroll
+          for (int r = 0; r < kBatch; ++r) {
+            const int64_t jr = j + r0 + r * kRows;
+            const float sum[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+            if (jr < a.nj && i < a.ni)
+              finish<E>(a, jr, i, sum, bias, residual[r]);
+          }
         }
       }
       wave_sync();
@@ -787,7 +810,10 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(AtomoProduct a) {
   const int64_t j = id / fours;
   const int i = (int)(id % fours) * 4;
   if (j >= a.nj) return;
+  const Four<typename E::Raw> bias = bias_of<E>(a, i);
+  const Four<typename E::Raw> residual = residual_of<E>(a, j, i);
   float sum[4] = {};
+#pragma unroll 4
   for (int part = 0; part < a.splits; ++part) {
     const float4 v = *(const float4*)(a.partial +
                                       ((int64_t)part * a.nj + j) * a.ld_part + i);
@@ -796,7 +822,7 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(AtomoProduct a) {
     sum[2] += v.z;
     sum[3] += v.w;
   }
-  finish<E>(a, j, i, sum);
+  finish<E>(a, j, i, sum, bias, residual);
 }
 
 // Few rows: the weight is read once, at the memory's rate, by waves that each
