@@ -17,6 +17,9 @@
 // a lane then holds four neighbouring i of one j, and stores them at once.
 //
 // Sums are fp32; an output is rounded once.
+//
+// Sizes decide the tile and in how many parts the reduction is made
+// (atomo_product_plan); few rows have a kernel of their own.
 
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -209,9 +212,9 @@ struct Stage {
     return kAll % kThreads != 0 && id >= kAll;
   }
 
-  // All of it lies in memory, but for rows from `rows` on (a multiple of four,
-  // where it lies across): another row is read in their place, which only
-  // reaches results that nobody keeps.
+  // All of it lies in memory, but for rows from `rows` on: others are read in
+  // their place, or, where it lies across, up to three elements that follow;
+  // both only reach results that nobody keeps.
   __device__ __forceinline__ void load_whole(const Raw* at, int64_t ld,
                                              int rows) {
     if constexpr (!kAcross) {
@@ -231,7 +234,7 @@ struct Stage {
         const int id = threadIdx.x + b * kThreads;
         if (idle(id)) break;
         const Raw* src = at + (int64_t)(id / (kRows / 4) * kC) * ld +
-                         min(id % (kRows / 4) * 4, rows - 4);
+                         min(id % (kRows / 4) * 4, (rows - 1) & ~3);
 #pragma unroll
         for (int e = 0; e < kC; ++e) {
           if constexpr (kC == 4) {
@@ -541,8 +544,12 @@ struct Work {
     steps = (ks + kK - 1) / kK;
     p = (const Raw*)a.p + (kAcrossP ? (int64_t)k0 * a.ldp + i0 : i0 * a.ldp + k0);
     q = (const Raw*)a.q + (kAcrossQ ? (int64_t)k0 * a.ldq + j0 : j0 * a.ldq + k0);
-    // steps that load_whole() may take
-    whole = (kAcrossP && rows_i % 4) || (kAcrossQ && rows_j % 4) ? 0 : ks / kK;
+    // Steps that load_whole() may take.  Blocks of four that pass the end of
+    // their row end in the next one: there has to be one.
+    const bool past_p = kAcrossP && rows_i % 4, past_q = kAcrossQ && rows_j % 4;
+    const bool next = !((past_p && a.ldp < 3) || (past_q && a.ldq < 3));
+    const int last = past_p || past_q ? min(ks, a.nk - 1 - k0) : ks;
+    whole = next ? last / kK : 0;
     // Neighbours start at different steps: rows of a power of two bytes put
     // all that one step reads on a few of L2's channels (dW of 8192 x 4096 x
     // 4096 bf16: 619 -> 322 us).  The order of the sum depends on the tile
@@ -656,7 +663,11 @@ __device__ __forceinline__ void write_tile(const AtomoProduct& a, int part,
 }
 
 // kI x kJ of the result by kWi x kWj waves; a tile of the reduction is 128
-// bytes of each row, double-buffered in LDS.  With several parts of the
+// bytes of each row, double-buffered in LDS.  8192 x 4096 x 4096 bf16, forward
+// / dx / dW: 314 / 301 / 296 us, 0.88 / 0.91 / 0.93 PFLOP/s, where a library's
+// products take 182 / 255 / 290.  Matrix instructions need 40 % of the time, LDS
+// reads and writes as much, and the barrier of each step keeps part of them
+// apart.  With several parts of the
 // reduction (`splits`) each leaves its fp32 sums for join_parts_kernel.
 template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
           int kWj, bool kTiny>
@@ -710,9 +721,12 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
 // The same for fp32 operands on the bf16 matrix instructions, 16 times as fast
 // as the fp32 ones: with x = a + b + c and y = a' + b' + c' (put_thirds) the
 // six products aa', ab', ba', bb', ac', ca' are xy but for 2^-25 of it, less
-// than fp32 loses by its sums.  2.7 times less time in matrix instructions
-// (128 x 9216 x 4096, forward / dx / dW: 100 / 109 / 139 us by fp32
-// instructions).  One buffer in LDS, so that three workgroups share a CU and
+// than fp32 loses by its sums.  2.7 times less time in matrix
+// instructions: 8192 x 4096 x 4096 forward in 1.4 ms, 0.2 PFLOP/s, above the
+// 0.157 of the fp32 ones; 128 x 9216 x 4096, forward / dx / dW, in 65 / 82 / 91
+// us (by fp32 instructions 100 / 109 / 139).  There the weight's 151 MB take
+// 27 us; splitting, LDS and matrix instructions as long each, and the barriers
+// keep them apart.  One buffer in LDS, so that three workgroups share a CU and
 // fill each other's waits.
 //
 // Where a sum comes out infinite or NaN (0 times a split infinity is NaN, and
@@ -802,7 +816,8 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
 
 constexpr int kThreads = 256;
 
-// the parts' sums, added in order, and the epilogue; a thread four neighbours
+// The parts' sums, added in order, and the epilogue; a thread four neighbours.
+// Bound by the memory: 16 parts of 128 x 4096 in 7.5 us.
 template <typename E>
 __global__ void __launch_bounds__(kThreads) join_parts_kernel(AtomoProduct a) {
   const int64_t fours = a.ld_part / 4;
@@ -825,7 +840,8 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(AtomoProduct a) {
   finish<E>(a, j, i, sum, bias, residual);
 }
 
-// Few rows: the weight is read once, at the memory's rate, by waves that each
+// Few rows, bound by the memory (1 x 9216 -> 4096 bf16 in 13 us, 5.7 TB/s; in
+// tiles 138 us): the weight is read once, by waves that each
 // take kN of its rows and all of x's kM; a lane takes every 64th 16 bytes.
 template <typename E, int kM, int kN>
 __global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
@@ -922,7 +938,8 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
 }
 
 // dp, and the sums of the columns of a block of rows.  64 lanes take 64
-// neighbouring vectors of a row, the waves every kDpWaves-th row.
+// neighbouring vectors of a row, the waves every kDpWaves-th row.  Bound by the
+// memory: 8192 x 4096 bf16 in 49 us, 4.1 TB/s; 128 rows by latency, 9 to 14 us.
 constexpr int kDpWaves = 16;
 
 template <typename E>
@@ -1072,10 +1089,8 @@ void product(const AtomoProduct& a, hipStream_t stream) {
       few_rows<E, 1>(a, stream);
     else if (a.nj <= 2)
       few_rows<E, 2>(a, stream);
-    else if (a.nj <= 4)
+    else if constexpr (E::kChunk == 4)
       few_rows<E, 4>(a, stream);
-    else
-      few_rows<E, 8>(a, stream);
     return;
   }
   if (a.plan == ATOMO_PLAN_TINY)
@@ -1109,8 +1124,41 @@ void linear_dp(const AtomoLinearDp& a, hipStream_t stream) {
                        a.columns, (Raw*)a.db);
 }
 
-int64_t tiles_of(const AtomoProduct& a, int size) {
-  return (int64_t)((a.ni + size - 1) / size) * ((a.nj + size - 1) / size);
+// What a step of 128 bytes of the reduction costs a workgroup, in us: alone on
+// its CU, where it waits for its loads, and as its share of a full one; by
+// type (fp32, 16 bits), form and tile (64, 128, 256).  Measured on products of
+// 16 to 8192 by 10 to 4096 by 500 to 9216; the choices that follow from it, and
+// what lies next to them:
+//   1024 x 1024 x 1024 bf16 forward: 64, one part 11 us; 128, four parts 20
+//   2048 x 2048 x 2048 bf16 forward: 128, one part 37 us; two parts 41
+//   512 x 512 x 4096 bf16 forward: 64, four parts 15 us; one part 31
+//   128 x 9216 -> 4096 fp32 forward: 128, 16 parts 63 us; 8 or 32 parts 75
+struct Step {
+  float alone, shared;
+};
+constexpr Step kStep[2][3][3] = {
+    {{{0.90f, 0.56f}, {1.95f, 1.50f}, {}},
+     {{1.15f, 0.57f}, {1.85f, 1.50f}, {}},
+     {{1.40f, 0.83f}, {1.90f, 1.60f}, {}}},
+    {{{0.55f, 0.29f}, {0.90f, 0.98f}, {2.40f, 2.40f}},
+     {{0.75f, 0.34f}, {0.95f, 1.05f}, {2.35f, 2.35f}},
+     {{0.95f, 0.60f}, {1.00f, 1.10f}, {2.30f, 2.30f}}}};
+constexpr float kTileEnd[3] = {0.25f, 1.4f, 6.f};  // a tile's epilogue
+
+float cost_of(const AtomoProduct& a, int tile, int64_t splits, int steps) {
+  constexpr int kCus = 256;
+  const int size = 64 << tile;
+  const int64_t tiles =
+      (int64_t)((a.ni + size - 1) / size) * ((a.nj + size - 1) / size);
+  const Step& step = kStep[a.type != ATOMO_F32][a.form][tile];
+  const float per_cu = (float)((tiles * splits + kCus - 1) / kCus);
+  float each = step.shared * per_cu;
+  if (each < step.alone) each = step.alone;
+  float us = each * (float)((steps + splits - 1) / splits) +
+             kTileEnd[tile] * per_cu;
+  // a launch more, and the sums written and read again at 5.5 TB/s
+  if (splits > 1) us += 3.5f + (float)a.ni * a.nj * splits * (8 / 5.5e6f);
+  return us;
 }
 
 }  // namespace
@@ -1126,45 +1174,42 @@ int64_t tiles_of(const AtomoProduct& a, int size) {
 extern "C" {
 
 void atomo_product_plan(AtomoProduct* a) {
-  constexpr int kCus = 256;
   a->splits = 1;
   a->k_part = a->nk;
-  if (a->form == ATOMO_FORWARD && a->nj <= 8) {
+  a->ld_part = (a->ni + 3) / 4 * 4;
+  a->bare = a->act == ATOMO_ACT_NONE && !a->bias && !a->residual && !a->slope;
+  // Beyond, the vector units bound it: 9216 -> 4096 for 2 / 4 rows, bf16 20 /
+  // 32 us, in tiles 21 / 21; fp32 for 4 / 8 rows 49 / 63 us, in tiles 56 / 56.
+  if (a->form == ATOMO_FORWARD && a->nj <= (a->type == ATOMO_F32 ? 4 : 2)) {
     a->plan = ATOMO_PLAN_FEW_ROWS;
     return;
   }
   // a vector of the reduction, or four rows that lie across, are read at once
-  const bool tiny = (a->form != ATOMO_GRAD_W && a->nk < 8) ||
-                    (a->form != ATOMO_FORWARD && a->ni < 4) ||
-                    (a->form == ATOMO_GRAD_W && a->nj < 4);
+  if ((a->form != ATOMO_GRAD_W && a->nk < 8) ||
+      (a->form != ATOMO_FORWARD && a->ni < 4) ||
+      (a->form == ATOMO_GRAD_W && a->nj < 4)) {
+    a->plan = ATOMO_PLAN_TINY;
+    return;
+  }
   const int step = kRowBytes / (a->type == ATOMO_F32 ? 4 : 2);
   const int steps = (a->nk + step - 1) / step;
-  // parts of four steps at least: below, joining costs more than it spreads
-  const int most = steps >= 8 ? steps / 4 : 1;
-  const int64_t t64 = tiles_of(*a, 64), t128 = tiles_of(*a, 128);
-  int64_t tiles = t128;
-  a->plan = ATOMO_PLAN_128;
-  if (tiny) {
-    a->plan = ATOMO_PLAN_TINY;
-    tiles = t64;
-  } else if (a->type != ATOMO_F32 && tiles_of(*a, 256) >= 192) {
-    a->plan = ATOMO_PLAN_256;
-    tiles = tiles_of(*a, 256);
-  } else if (t128 * most < kCus) {
-    a->plan = ATOMO_PLAN_64;
-    tiles = t64;
-  }
-  // one workgroup a CU of the largest tiles, two of the others
-  int64_t splits = (a->plan == ATOMO_PLAN_256 ? kCus : 2 * kCus) / tiles;
-  splits = splits < most ? splits : most;
+  float least = 0.f;
+  int64_t splits = 0;
+  for (int tile = 0; tile < (a->type == ATOMO_F32 ? 2 : 3); ++tile)
+    for (const int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (n > 1 && n * 4 > steps) break;  // parts of four steps at least
+      const float us = cost_of(*a, tile, n, steps);
+      if (splits && us >= least) continue;
+      least = us;
+      splits = n;
+      a->plan = ATOMO_PLAN_64 + tile;
+    }
   if (splits > 1) {
     const int part = (int)((steps + splits - 1) / splits);
     a->k_part = part * step;
     a->splits = (steps + part - 1) / part;
+    a->bare = 1;
   }
-  a->ld_part = (a->ni + 3) / 4 * 4;
-  a->bare = a->splits > 1 || (a->act == ATOMO_ACT_NONE && !a->bias &&
-                              !a->residual && !a->slope);
 }
 
 void atomo_product_launch(const AtomoProduct* a, hipStream_t stream) {

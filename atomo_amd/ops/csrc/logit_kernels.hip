@@ -318,6 +318,14 @@ __device__ uint64_t cut_list(uint64_t* list, int n, int k) {
 // The k-th best of the maxima of all loads bounds the k-th best class from
 // below, for k classes reach it; so only the few chunks (about k) that reach
 // it are read again, out of a cache, and of their classes those that do.
+//
+// Bound by the memory, and in 16 bits nearly as much by the vector units, at
+// some ten instructions an element, four of them the exponential.  4096 x
+// 32000 fp32: without alternatives 92 us, 5.7 TB/s, with 64 of them 119 us,
+// 4.4 TB/s; 2048 x 50021 bf16 in padded rows, 8 of them: 54 us, 3.8 TB/s.  (A
+// large copy reaches 5.5 TB/s.)  Looking every class up against a bar while it
+// is read took 264 and 108 us.  Rows of equal or rising logits reach any bar
+// everywhere: 512 x 20000 fp32 take up to 106 us, else 10.
 constexpr int kParts = 4;    // 16-byte loads in flight for each thread
 constexpr int kChunks = 16;  // between two selections
 
@@ -525,7 +533,9 @@ __global__ void __launch_bounds__(kThreads)
 
 // Joins a row's parts: one workgroup a row.  A part's last key, where it has
 // k, is a bar for all of them; so is the least of the parts' d-th keys, where
-// d keys of each are k together, and mostly the higher one.
+// d keys of each are k together, and mostly the higher one.  Bound by latency:
+// one row of 131072 bf16 with 20 alternatives takes 10 us in 16 parts and 5 us
+// here, 22 us in all with 128.
 constexpr int kMostSplits = ATOMO_LOGIT_MAX_SPLITS;
 constexpr int kJoin = 256;
 
@@ -824,7 +834,11 @@ __device__ __forceinline__ void write_zeros(typename E::Raw* g, int first,
 }
 
 // Loss and, where it is wanted, gradient of a row that fits a workgroup's
-// registers, kLoads 16-byte loads a thread: the logits are read once.
+// registers, kLoads 16-byte loads a thread: the logits are read once.  Bound by
+// the memory: 4096 x 65536 bf16 with an eighth of the rows ignored in 223 us,
+// 4.5 TB/s.  Four waves a SIMD, that is two workgroups of 512 a CU, matter: one
+// reads while the other sums (190 registers, one workgroup: 351 us).  Reading
+// the next row ahead into registers instead spilled, 400 us.
 template <typename E, int kThreads, int kLoads>
 __global__ void __launch_bounds__(kThreads)
     __attribute__((amdgpu_waves_per_eu(4))) distill_fused_kernel(Distill a) {
@@ -922,7 +936,9 @@ __global__ void __launch_bounds__(kThreads)
 
 constexpr int kSweep = 256;
 
-// The sums of a part of a row, and of a whole one the loss.
+// The sums of a part of a row, and of a whole one the loss: a sweep with the
+// running maximum.  Bound by the memory: 4096 x 32000 fp32 with an eighth of
+// the rows ignored in 89 us, 5.2 TB/s; 1001 x 50021 fp16 in 28 us, 3.6 TB/s.
 template <typename E>
 __global__ void __launch_bounds__(kSweep) distill_sums_kernel(Distill a) {
   constexpr int kV = E::kVec;
@@ -992,7 +1008,7 @@ __device__ __forceinline__ Sums row_sums(const Distill& a, int64_t row) {
   return wave_join(st, a.inv_tau);
 }
 
-// The split rows' losses from their sums: one wave a row.
+// The split rows' losses from their sums: one wave a row, bound by latency.
 template <typename E>
 __global__ void __launch_bounds__(WAVE) distill_loss_kernel(Distill a) {
   const int64_t row = grid_row(1);
@@ -1009,7 +1025,8 @@ __global__ void __launch_bounds__(WAVE) distill_loss_kernel(Distill a) {
   if (threadIdx.x == 0) a.row_loss[row] = loss;
 }
 
-// The gradient of a part of a row from the row's sums.
+// The gradient of a part of a row from the row's sums.  Bound by the memory:
+// 1001 x 50021 fp16 in 41 us, 4.9 TB/s.
 template <typename E>
 __global__ void __launch_bounds__(kSweep) distill_grad_kernel(Distill a) {
   constexpr int kV = E::kVec;
@@ -1069,6 +1086,8 @@ __global__ void __launch_bounds__(kSweep) distill_grad_kernel(Distill a) {
   if (wave == 0) teacher.patch<E>(a, st, pt, p1, ct, c1, g, first, end);
 }
 
+// Rows that count, and the rows' losses added up in a fixed order: one
+// workgroup, bound by latency (4096 rows: 3 and 5 us).
 __global__ void __launch_bounds__(1024)
     count_rows_kernel(const int64_t* __restrict__ labels, int64_t rows,
                       int64_t ignore, float* __restrict__ inverse) {

@@ -160,6 +160,19 @@ def test_layouts(m, k, n, dtype):
         assert torch.equal(gx.cpu(), (dy.double() @ w.double()).to(dtype))
         assert torch.equal(gw.cpu(), (dy.double().t() @ x.double()).to(dtype))
         assert torch.equal(gr.cpu(), dy)
+    # rows that share their elements, and end where their memory ends
+    def sliding(rows, columns, seed):
+        flat = _grid((rows + columns - 1,), seed, dtype)
+        return (flat.as_strided((rows, columns), (1, 1)),
+                flat.cuda().as_strided((rows, columns), (1, 1)))
+
+    (hx, sx), (hd, sdy) = sliding(m, k, 8), sliding(m, n, 9)
+    cx, cw = sx.detach().requires_grad_(), w.cuda().requires_grad_()
+    y = linear_ops.linear_act(cx, cw)
+    gx, gw = torch.autograd.grad(y, (cx, cw), sdy)
+    assert torch.equal(y.cpu(), (hx.double() @ w.double().t()).to(dtype))
+    assert torch.equal(gx.cpu(), (hd.double() @ w.double()).to(dtype))
+    assert torch.equal(gw.cpu(), (hd.double().t() @ hx.double()).to(dtype))
     # one row for all, and a gradient that is one number
     cx = x[:1].cuda().requires_grad_()
     cw = w.cuda().requires_grad_()
