@@ -13,6 +13,10 @@ Kernels (sources in ops/csrc/, reference hot-spot map SURVEY §2.10):
   * svd_decode_acc — fused u·diag(s)·vT rank-k reconstruction accumulated
     over ALL workers' packets in one output sweep.
   * fused_sgd — scale+weight-decay+momentum+apply in one flat sweep.
+  * linear_act — matrix product with bias, activation and residual in its
+    epilogue, forward and backward (MFMA; fp32 as three bf16 parts).
+  * label_logprobs — log probability, entropy and top classes of each row.
+  * distill_loss — loss against a teacher's top logits, with its gradient.
 """
 
 from __future__ import annotations
