@@ -44,14 +44,16 @@ int64_t row_stride(const Tensor& t) {
   return t.size(0) > 1 ? t.stride(0) : t.size(1);
 }
 
-void product(AtomoProduct a, const Tensor& like) {
-  atomo_product_plan(&a);
-  Tensor partial;
-  if (a.splits > 1) {
-    partial = torch::empty({a.splits, a.nj, a.ld_part},
-                           like.options().dtype(torch::kFloat32));
-    a.partial = partial.data_ptr<float>();
-  }
+// fp32 numbers that a planned product needs to put its parts
+int64_t parts_of(const AtomoProduct& a) {
+  return a.splits > 1 ? a.splits * a.nj * a.ld_part : 0;
+}
+
+Tensor floats(int64_t n, const Tensor& like) {
+  return n ? torch::empty({n}, like.options().dtype(torch::kFloat32)) : Tensor();
+}
+
+void product(const AtomoProduct& a) {
   atomo_product_launch(&a, cur_stream());
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
@@ -103,7 +105,10 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       a.type = type_of(x);
       a.form = ATOMO_FORWARD;
       a.act = (int)act;
-      product(a, x);
+      atomo_product_plan(&a);
+      const Tensor partial = floats(parts_of(a), x);
+      a.partial = partial.defined() ? partial.data_ptr<float>() : nullptr;
+      product(a);
     }
     ctx->saved_data["train"] = train;
     ctx->saved_data["bias"] = bias.defined();
@@ -141,61 +146,75 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       if (want_b) db = torch::zeros({n}, x.options());
       return {dx, dw, db, dr, Tensor(), Tensor()};
     }
-    Tensor dp = dy;
+    // What the three steps need in between lies in one piece of memory, in
+    // turn: the products' parts and db's block sums.
     const bool make_dp = slope.defined() && (want_x || want_w);
+    AtomoProduct px{}, pw{};
+    int64_t work = 0;
+    if (want_x) {
+      px.form = ATOMO_GRAD_X;
+      px.type = type;
+      px.ni = (int)k;
+      px.nj = (int)m;
+      px.nk = (int)n;
+      atomo_product_plan(&px);
+      work = std::max(work, parts_of(px));
+    }
+    if (want_w) {
+      pw.form = ATOMO_GRAD_W;
+      pw.type = type;
+      pw.ni = (int)k;
+      pw.nj = (int)n;
+      pw.nk = (int)m;
+      atomo_product_plan(&pw);
+      work = std::max(work, parts_of(pw));
+    }
+    AtomoLinearDp d{};
+    // blocks of 128 rows (8 for each of 16 waves) or more, 1024 at most
+    d.block_rows = (int)std::max<int64_t>(128, (m + 1023) / 1024);
+    d.row_blocks = (int)((m + d.block_rows - 1) / d.block_rows);
+    if (want_b && d.row_blocks > 1) work = std::max(work, d.row_blocks * n);
+    const Tensor between = floats(work, x);
+    float* partial = between.defined() ? between.data_ptr<float>() : nullptr;
+
+    Tensor dp = dy;
     if (make_dp || want_b) {
-      AtomoLinearDp d{};
+      if (make_dp) dp = torch::empty({m, n}, x.options());
+      if (want_b) db = torch::empty({n}, x.options());
       d.dy = dy.data_ptr();
       d.ld_dy = row_stride(dy);
       d.slope = slope.defined() ? slope.data_ptr() : nullptr;
       d.by_output = ctx->saved_data["by_output"].toBool();
+      d.dp = make_dp ? dp.data_ptr() : nullptr;
+      d.db = want_b ? db.data_ptr() : nullptr;
+      d.partial = partial;
       d.rows = (int)m;
       d.columns = (int)n;
       d.type = type;
-      if (make_dp) dp = torch::empty({m, n}, x.options());
-      d.dp = make_dp ? dp.data_ptr() : nullptr;
-      // blocks of 128 rows (8 for each of 16 waves) or more, 1024 at most
-      d.block_rows = (int)std::max<int64_t>(128, (m + 1023) / 1024);
-      d.row_blocks = (int)((m + d.block_rows - 1) / d.block_rows);
-      Tensor partial;
-      if (want_b) {
-        db = torch::empty({n}, x.options());
-        d.db = db.data_ptr();
-        if (d.row_blocks > 1) {
-          partial = torch::empty({d.row_blocks, n},
-                                 x.options().dtype(torch::kFloat32));
-          d.partial = partial.data_ptr<float>();
-        }
-      }
       atomo_linear_dp_launch(&d, cur_stream());
       C10_HIP_KERNEL_LAUNCH_CHECK();
     }
-    AtomoProduct a{};
-    a.type = type;
-    a.act = ATOMO_ACT_NONE;
-    a.q = dp.data_ptr();
-    a.ldq = row_stride(dp);
-    a.ni = (int)k;
-    a.ldo = k;
     if (want_x) {
       dx = torch::empty({m, k}, x.options());
-      a.p = weight.data_ptr();
-      a.ldp = row_stride(weight);
-      a.out = dx.data_ptr();
-      a.nj = (int)m;
-      a.nk = (int)n;
-      a.form = ATOMO_GRAD_X;
-      product(a, x);
+      px.p = weight.data_ptr();
+      px.ldp = row_stride(weight);
+      px.q = dp.data_ptr();
+      px.ldq = row_stride(dp);
+      px.out = dx.data_ptr();
+      px.ldo = k;
+      px.partial = partial;
+      product(px);
     }
     if (want_w) {
       dw = torch::empty({n, k}, x.options());
-      a.p = x.data_ptr();
-      a.ldp = row_stride(x);
-      a.out = dw.data_ptr();
-      a.nj = (int)n;
-      a.nk = (int)m;
-      a.form = ATOMO_GRAD_W;
-      product(a, x);
+      pw.p = x.data_ptr();
+      pw.ldp = row_stride(x);
+      pw.q = dp.data_ptr();
+      pw.ldq = row_stride(dp);
+      pw.out = dw.data_ptr();
+      pw.ldo = k;
+      pw.partial = partial;
+      product(pw);
     }
     return {dx, dw, db, dr, Tensor(), Tensor()};
   }

@@ -40,8 +40,8 @@ struct AtomoProduct {
   int64_t ldp, ldq, ldo, ldr, ld_part;
   int ni, nj, nk;
   int type, form, act;
-  // by atomo_product_plan, from all above but `partial`; `bare`: the tiles
-  // have no epilogue
+  // by atomo_product_plan, from type, form, act, the sizes and which of bias,
+  // residual and slope there are; `bare`: the tiles have no epilogue
   int plan, splits, k_part, bare;
 };
 
