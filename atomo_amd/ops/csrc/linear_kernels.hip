@@ -441,30 +441,33 @@ __device__ __forceinline__ float slope_of(uint16_t r) {
                       : (float)((int)r - 8192) * (1.f / 32768.f);
 }
 
-// four neighbours of a row, at the alignment of one
-template <typename Raw>
-struct Four {
-  Raw v[4];
+// neighbours in a row, at the alignment of one
+template <typename Raw, int kN>
+struct Some {
+  Raw v[kN];
 } __attribute__((packed, aligned(sizeof(Raw))));
-
-// the first n of four
 template <typename Raw>
-__device__ __forceinline__ Four<Raw> load_four(const Raw* at, int n) {
-  Four<Raw> f = {};
-  if (n >= 4) return *(const Four<Raw>*)at;
+using Four = Some<Raw, 4>;
+
+// the first n of them
+template <int kN, typename Raw>
+__device__ __forceinline__ Some<Raw, kN> load_some(const Raw* at, int n) {
+  Some<Raw, kN> f = {};
+  if (n >= kN) return *(const Some<Raw, kN>*)at;
 #pragma unroll
-  for (int e = 0; e < 3; ++e)
+  for (int e = 0; e < kN - 1; ++e)
     if (e < n) f.v[e] = at[e];
   return f;
 }
-template <typename Raw>
-__device__ __forceinline__ void store_four(Raw* at, int n, const Four<Raw>& f) {
-  if (n >= 4) {
-    *(Four<Raw>*)at = f;
+template <int kN, typename Raw>
+__device__ __forceinline__ void store_some(Raw* at, int n,
+                                           const Some<Raw, kN>& f) {
+  if (n >= kN) {
+    *(Some<Raw, kN>*)at = f;
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 3; ++e)
+  for (int e = 0; e < kN - 1; ++e)
     if (e < n) at[e] = f.v[e];
 }
 
@@ -488,21 +491,21 @@ __device__ __forceinline__ void finish(const AtomoProduct& a, int64_t j, int i,
     if (a.residual) h += E::widen(residual.v[e]);
     y.v[e] = E::narrow(h);
   }
-  store_four((Raw*)a.out + j * a.ldo + i, a.ni - i, y);
-  if (a.slope) store_four((Slope*)a.slope + j * a.ni + i, a.ni - i, s);
+  store_some<4>((Raw*)a.out + j * a.ldo + i, a.ni - i, y);
+  if (a.slope) store_some<4>((Slope*)a.slope + j * a.ni + i, a.ni - i, s);
 }
 
 template <typename E>
 __device__ __forceinline__ Four<typename E::Raw> bias_of(const AtomoProduct& a,
                                                          int i) {
   if (!a.bias || i >= a.ni) return {};
-  return load_four((const typename E::Raw*)a.bias + i, a.ni - i);
+  return load_some<4>((const typename E::Raw*)a.bias + i, a.ni - i);
 }
 template <typename E>
 __device__ __forceinline__ Four<typename E::Raw> residual_of(
     const AtomoProduct& a, int64_t j, int i) {
   if (!a.residual || i >= a.ni || j >= a.nj) return {};
-  return load_four((const typename E::Raw*)a.residual + j * a.ldr + i, a.ni - i);
+  return load_some<4>((const typename E::Raw*)a.residual + j * a.ldr + i, a.ni - i);
 }
 
 // lanes of one wave read in LDS what others of it wrote
@@ -590,7 +593,7 @@ __device__ __forceinline__ void put_bare(const AtomoProduct& a, int part,
   }
   const Four<Raw> y = {{E::narrow(v.x), E::narrow(v.y), E::narrow(v.z),
                         E::narrow(v.w)}};
-  store_four((Raw*)a.out + j * a.ldo + i, a.ni - i, y);
+  store_some<4>((Raw*)a.out + j * a.ldo + i, a.ni - i, y);
 }
 
 // A wave's sums, from row i0 and column j0 of the result on, to the epilogue
@@ -644,11 +647,22 @@ __device__ __forceinline__ void write_tile(const AtomoProduct& a, int part,
         for (int r0 = 0; r0 < 32; r0 += kRows * kBatch) {
           float4 v[kBatch];
           Four<typename E::Raw> residual[kBatch];
+          const auto load = [&](int n) {
 #pragma unroll
-          for (int r = 0; r < kBatch; ++r) {
-            residual[r] = residual_of<E>(a, j + r0 + r * kRows, i);
+            for (int r = 0; r < kBatch; ++r)
+              residual[r] = load_some<4>(
+                  (const typename E::Raw*)a.residual +
+                      min(j + r0 + r * kRows, (int64_t)a.nj - 1) * a.ldr + i,
+                  n);
+          };
+          // whole ones apart, without a branch in between
+          if (a.residual && i + 4 <= a.ni)
+            load(4);
+          else if (a.residual && i < a.ni)
+            load(a.ni - i);
+#pragma unroll
+          for (int r = 0; r < kBatch; ++r)
             v[r] = *(const float4*)(from + (r0 + r * kRows) * kPitch);
-          }
 #pragma unroll
           for (int r = 0; r < kBatch; ++r) {
             const int64_t jr = j + r0 + r * kRows;
@@ -937,94 +951,81 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
   }
 }
 
-// dp, and the sums of the columns of a block of rows.  64 lanes take 64
-// neighbouring vectors of a row, the waves every kDpWaves-th row.  Bound by the
-// memory: 8192 x 4096 bf16 in 49 us, 4.1 TB/s; 128 rows by latency, 9 to 14 us.
+// dp, and the sums of the columns of a block of rows.  64 lanes take 64 times
+// kV neighbours of a row, the waves every kDpWaves-th row.  Bound by the
+// memory: 8192 x 4096 bf16 in 45 us, 4.5 TB/s.  kV is four, or one where four
+// would leave most CUs without a workgroup: 128 x 4096 fp32 in 6.5 us (by
+// fours 13), 128 x 800 in 5 (9).
 constexpr int kDpWaves = 16;
 
-template <typename E>
+template <typename E, int kV>
 __global__ void __launch_bounds__(kDpWaves * 64)
-    linear_dp_kernel(const typename E::Raw* __restrict__ dy, int64_t ld_dy,
-                     const void* __restrict__ slope, int by_output,
-                     typename E::Raw* __restrict__ dp,
-                     float* __restrict__ partial,
-                     typename E::Raw* __restrict__ db, int rows, int columns,
-                     int block_rows) {
+    linear_dp_kernel(AtomoLinearDp a) {
   using Raw = typename E::Raw;
   using Slope = typename E::Slope;
-  __shared__ float lds[kDpWaves][64 * 4];
+  __shared__ float lds[kDpWaves][64 * kV];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int c = (blockIdx.x * 64 + lane) * 4;
-  const int n = min(4, columns - c);
-  const int first = blockIdx.y * block_rows;
-  const int last = min(rows, first + block_rows);
-  float sum[4] = {};
+  const int c = (blockIdx.x * 64 + lane) * kV;
+  const int n = min(kV, a.columns - c);
+  const int first = blockIdx.y * a.block_rows;
+  const int last = min(a.rows, first + a.block_rows);
+  const Raw* dy = (const Raw*)a.dy;
+  const bool by_output = a.slope && a.by_output;
+  const bool by_slope = a.slope && !a.by_output;
+  float sum[kV] = {};
   // four rows are read before the first is used
   constexpr int kDepth = 4;
   for (int r0 = first + wave; r0 < last; r0 += kDpWaves * kDepth) {
     if (n <= 0) break;
-    Four<Raw> v[kDepth], y[kDepth];
-    Four<Slope> s[kDepth];
+    Some<Raw, kV> v[kDepth], y[kDepth];
+    Some<Slope, kV> s[kDepth];
+    const auto load = [&](int n) {
 #pragma unroll
-    for (int u = 0; u < kDepth; ++u) {
-      const int64_t r = min(r0 + u * kDpWaves, last - 1);
-      const Raw* from = dy + r * ld_dy + c;
-      const int64_t at = r * columns + c;
-      if (n == 4) {
-        v[u] = *(const Four<Raw>*)from;
-        if (slope && by_output) y[u] = *(const Four<Raw>*)((const Raw*)slope + at);
-        if (slope && !by_output)
-          s[u] = *(const Four<Slope>*)((const Slope*)slope + at);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e) {
-          if (e >= n) break;
-          v[u].v[e] = from[e];
-          if (slope && by_output) y[u].v[e] = ((const Raw*)slope)[at + e];
-          if (slope && !by_output) s[u].v[e] = ((const Slope*)slope)[at + e];
-        }
+      for (int u = 0; u < kDepth; ++u) {
+        const int64_t r = min(r0 + u * kDpWaves, last - 1);
+        const int64_t at = r * a.columns + c;
+        v[u] = load_some<kV>(dy + r * a.ld_dy + c, n);
+        if (by_output) y[u] = load_some<kV>((const Raw*)a.slope + at, n);
+        if (by_slope) s[u] = load_some<kV>((const Slope*)a.slope + at, n);
       }
-    }
+    };
+    // apart, so that whole ones are read without a branch in between
+    if (n == kV)
+      load(kV);
+    else
+      load(n);
 #pragma unroll
     for (int u = 0; u < kDepth; ++u) {
       const int r = r0 + u * kDpWaves;
       if (r >= last) break;
-      const int64_t at = (int64_t)r * columns + c;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (e >= n) break;
+      for (int e = 0; e < kV; ++e) {
         float d = E::widen(v[u].v[e]);
-        if (slope && by_output)
+        if (by_output)
           d = E::widen(y[u].v[e]) <= 0.f ? 0.f : d;
-        else if (slope)
+        else if (by_slope)
           d *= slope_of(s[u].v[e]);
         v[u].v[e] = E::narrow(d);
         sum[e] += d;
       }
-      if (!dp) continue;
-      if (n == 4) {
-        *(Four<Raw>*)(dp + at) = v[u];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (e < n) dp[at + e] = v[u].v[e];
-      }
+      if (a.dp)
+        store_some<kV>((Raw*)a.dp + (int64_t)r * a.columns + c, n, v[u]);
     }
   }
-  if (!partial && !db) return;
+  if (!a.db) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) lds[wave][lane * 4 + e] = sum[e];
+  for (int e = 0; e < kV; ++e) lds[wave][lane * kV + e] = sum[e];
   __syncthreads();
-  if (threadIdx.x < 256) {
+  if (threadIdx.x < 64 * kV) {
     float all = 0.f;
 #pragma unroll
     for (int w = 0; w < kDpWaves; ++w) all += lds[w][threadIdx.x];
-    const int column = blockIdx.x * 256 + threadIdx.x;
-    if (column < columns) {
-      if (db)
-        db[column] = E::narrow(all);
+    const int column = blockIdx.x * 64 * kV + threadIdx.x;
+    if (column < a.columns) {
+      if (a.row_blocks == 1)
+        ((Raw*)a.db)[column] = E::narrow(all);
       else
-        partial[(int64_t)blockIdx.y * columns + column] = all;
+        a.partial[(int64_t)blockIdx.y * a.columns + column] = all;
     }
   }
 }
@@ -1109,19 +1110,24 @@ void product(const AtomoProduct& a, hipStream_t stream) {
   }
 }
 
+template <typename E, int kV>
+void launch_dp(const AtomoLinearDp& a, hipStream_t stream) {
+  const int wide = 64 * kV;
+  hipLaunchKernelGGL((linear_dp_kernel<E, kV>),
+                     dim3((a.columns + wide - 1) / wide, a.row_blocks),
+                     dim3(kDpWaves * 64), 0, stream, a);
+}
+
 template <typename E>
 void linear_dp(const AtomoLinearDp& a, hipStream_t stream) {
-  using Raw = typename E::Raw;
-  const bool join = a.db && a.row_blocks > 1;
-  hipLaunchKernelGGL(
-      (linear_dp_kernel<E>), dim3((a.columns + 255) / 256, a.row_blocks),
-      dim3(kDpWaves * 64), 0, stream, (const Raw*)a.dy, a.ld_dy, a.slope,
-      a.by_output, (Raw*)a.dp, join ? a.partial : nullptr,
-      join ? nullptr : (Raw*)a.db, a.rows, a.columns, a.block_rows);
-  if (join)
+  if ((int64_t)(a.columns + 255) / 256 * a.row_blocks < 128)
+    launch_dp<E, 1>(a, stream);
+  else
+    launch_dp<E, 4>(a, stream);
+  if (a.db && a.row_blocks > 1)
     hipLaunchKernelGGL((linear_db_kernel<E>), dim3((a.columns + 63) / 64),
                        dim3(kDpWaves * 64), 0, stream, a.partial, a.row_blocks,
-                       a.columns, (Raw*)a.db);
+                       a.columns, (typename E::Raw*)a.db);
 }
 
 // What a step of 128 bytes of the reduction costs a workgroup, in us: alone on
