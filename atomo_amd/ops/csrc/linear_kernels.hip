@@ -737,7 +737,7 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
 // six products aa', ab', ba', bb', ac', ca' are xy but for 2^-25 of it, less
 // than fp32 loses by its sums.  2.7 times less time in matrix
 // instructions: 8192 x 4096 x 4096 forward in 1.4 ms, 0.2 PFLOP/s, above the
-// 0.157 of the fp32 ones; 128 x 9216 x 4096, forward / dx / dW, in 65 / 82 / 91
+// 0.157 of the fp32 ones; 128 x 9216 x 4096, forward / dx / dW, in 63 / 72 / 72
 // us (by fp32 instructions 100 / 109 / 139).  There the weight's 151 MB take
 // 27 us; splitting, LDS and matrix instructions as long each, and the barriers
 // keep them apart.  One buffer in LDS, so that three workgroups share a CU and
@@ -1202,7 +1202,7 @@ void atomo_product_plan(AtomoProduct* a) {
   float least = 0.f;
   int64_t splits = 0;
   for (int tile = 0; tile < (a->type == ATOMO_F32 ? 2 : 3); ++tile)
-    for (const int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    for (const int n : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32}) {
       if (n > 1 && n * 4 > steps) break;  // parts of four steps at least
       const float us = cost_of(*a, tile, n, steps);
       if (splits && us >= least) continue;
