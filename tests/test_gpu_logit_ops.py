@@ -135,6 +135,13 @@ def test_logprobs_labels_outside_and_other_stream():
     assert none.top_index.shape == (0, 3)
 
 
+@pytest.mark.parametrize("classes,dtype", [(4300001, F32), (8500003, BF16)])
+@pytest.mark.parametrize("mask", [None, "ties"])
+def test_logprobs_of_parts_with_several_selections(classes, dtype, mask):
+    z, cuda = _logits(2, classes, dtype, seed=9, mask=mask)
+    _check_logprobs(z, cuda, torch.tensor([classes - 1, -100]), 33)
+
+
 def test_more_rows_than_one_dimension_of_a_grid():
     rows, classes = 300001, 3
     z, cuda = _logits(rows, classes, F32)
@@ -264,6 +271,57 @@ def test_distill_sizes(rows, classes, dtype):
         value, index = _teacher(rows, classes, k)
         _check_distill(z, cuda, value, index, y, 2.0, 0.7)
         _check_distill(z, cuda, value, index, None, 1.0, 1.0, "sum")
+
+
+@pytest.mark.parametrize("classes,dtype", [
+    (4097, F32), (9000, BF16), (16385, F32), (40001, BF16), (32770, F32),
+    (70001, BF16), (131072, BF16), (65537, F32), (131073, BF16), (9001, F16)])
+def test_distill_long_rows_in_registers(classes, dtype):
+    """Enough rows that each has a workgroup; lengths around what 64, 256, 512
+    and 1024 threads hold, and beyond."""
+    rows = 129
+    z, cuda = _logits(rows, classes, dtype, seed=classes)
+    z[3] = -math.inf
+    z[4, 1:] = -math.inf
+    cuda.copy_(z)
+    value, index = _teacher(rows, classes, 5)
+    y = _labels(rows, classes)
+    leaf = cuda.detach().requires_grad_()
+    args = (value.cuda(), index.cuda(), y.cuda())
+    loss = logit_ops.distill_loss(leaf, *args, temperature=2.0, weight=0.7)
+    (grad,) = torch.autograd.grad(loss, leaf)
+    # against the same in 64 bits, on the device for speed
+    wide = z[5:].cuda().double()
+    count = int((y != -100).sum())
+    q = torch.zeros_like(wide).scatter_(1, args[1][5:], torch.softmax(args[0][5:].double() / 2, 1))
+    at = args[2][5:].clamp_min(0)[:, None]
+    hot = torch.zeros_like(wide).scatter_(1, at, 1.0)
+    pt, p1 = torch.softmax(wide / 2, 1), torch.softmax(wide, 1)
+    keep = (args[2][5:] != -100).double()[:, None] / count
+    want = (1.4 * (pt - q) + 0.3 * (p1 - hot)) * keep
+    size = (1.4 * (pt + q) + 0.3 * (p1 + hot)) * keep
+    u = U * (_steps(classes, _spread(z)) + 10 + _spread(value))
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    tol = 2 * u * size + half * want.abs() + tiny
+    assert ((grad[5:].double() - want).abs() <= tol).all()
+    assert (grad[3] == 0).all() and (grad[args[2] == -100] == 0).all()
+    few = z[:5].clone()
+    cpu = logit_ops.distill_loss(few, value[:5], index[:5], y[:5], temperature=2.0,
+                                 weight=0.7, reduction="none")
+    gpu = logit_ops.distill_loss(cuda[:5], *(t[:5] for t in args), temperature=2.0,
+                                 weight=0.7, reduction="none").cpu()
+    # a handful of rows goes another way
+    loss_size, _ = _terms(few, value[:5], index[:5], y[:5], 2.0, 0.7)
+    ok = _same_odd(gpu, cpu)
+    assert ((gpu - cpu).abs() <= 2 * u * loss_size)[ok].all()
+    rest = torch.cat([cpu.double(), (
+        2.8 * (torch.special.xlogy(q, q) - q * torch.log_softmax(wide / 2, 1)).sum(1)
+        - 0.3 * torch.log_softmax(wide, 1).gather(1, at)[:, 0]).cpu() * (y[5:] != -100)])
+    if torch.isfinite(rest).all():
+        total, _ = _terms(z, value, index, y, 2.0, 0.7)
+        bound = (2 * u + U * (rows / 64 + 64)) * (total * (y != -100)).sum() / count
+        assert abs(float(loss) - float(rest.sum() / count)) <= bound
 
 
 @pytest.mark.parametrize("tau,weight,reduction,up", [
