@@ -123,9 +123,10 @@ def distill_loss(
     ``weight``, and against ``labels`` (...) with ``1 - weight``.
 
     ``temperature`` lies in 0.01..100.  The values may be logits or log
-    probabilities: a constant added to a row changes nothing.  k is at most 128; an entry of -inf is absent, and its
-    index is not looked at.  Any other index outside 0..classes-1 makes the
-    row NaN, and so does such a label, except ``ignore_index``: that row has
+    probabilities: a constant added to a row changes nothing.  k is at
+    most 128; an entry of -inf is absent, and its index is not looked at.  Any
+    other index outside 0..classes-1 makes the row NaN, its gradient too, as do
+    a value of NaN or +inf and such a label, except ``ignore_index``: that row has
     no loss, no gradient, and is not counted in the mean (of no rows: 0).
     ``labels`` may be given with ``weight=1`` to leave rows out, and has to be
     with any other weight; with ``weight=0`` the teacher is not looked at.
@@ -236,7 +237,7 @@ class _DistillOracle(torch.autograd.Function):
             log_p = _log_softmax(z.double() / tau)
             kd = (_times(q, q.log()) - _times(q, log_p)).sum(1)
             bad = torch.where((there & ~inside).any(1), math.nan, 0.0)
-            bad = bad + torch.where(value.isnan().any(1), math.nan, 0.0)
+            bad = bad + torch.where(t.isnan().any(1), math.nan, 0.0)
             any_q = there.any(1, keepdim=True)
             row += weight * tau * tau * (kd + bad)
             grad += weight * tau * (

@@ -361,6 +361,15 @@ def test_distill_wrong_entries(classes):
     _check_distill(z, cuda, value, index, y, 2.0, 0.6, "none")
 
 
+@pytest.mark.parametrize("classes", [50, 20000])
+def test_distill_infinite_teacher(classes):
+    z, cuda = _logits(3, classes, F32)
+    value, index = _teacher(3, classes, 4)
+    value[1, 2] = math.inf
+    y = torch.tensor([0, 1, -100])
+    _check_distill(z, cuda, value, index, y, 2.0, 0.6, "none")
+
+
 @pytest.mark.parametrize("pad,offset", [(1, 0), (5, 3), (64, 8)])
 def test_distill_strides(pad, offset):
     for dtype in (F32, F16):

@@ -192,6 +192,17 @@ def test_distill_absent_and_wrong_entries():
     assert bad.isnan().tolist() == [False, True, True, False, False]
 
 
+def test_distill_infinite_teacher():
+    """A teacher's +inf leaves no distribution: loss and gradient of the row
+    are NaN throughout."""
+    z = _logits(2, 6).requires_grad_()
+    value = torch.tensor([[1.0, math.inf], [1.0, 0.0]])
+    loss = logit_ops.distill_loss(z, value, torch.tensor([[0, 1], [0, 1]]), reduction="none")
+    loss.sum().backward()
+    assert loss.isnan().tolist() == [True, False]
+    assert z.grad[0].isnan().all() and torch.isfinite(z.grad[1]).all()
+
+
 def test_distill_masked_student():
     inf = math.inf
     z = torch.tensor([[-inf] * 3, [0.0, -inf, 1.0], [0.0, -inf, 1.0]], requires_grad=True)
