@@ -22,6 +22,14 @@ using torch::autograd::variable_list;
 
 hipStream_t cur_stream() { return c10::hip::getCurrentHIPStream().stream(); }
 
+// the capture that a stream's work goes to, 0 for none
+int64_t capture_of(hipStream_t stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_HIP_CHECK(hipStreamGetCaptureInfo(stream, &status, &id));
+  return status == hipStreamCaptureStatusNone ? 0 : (int64_t)id;
+}
+
 int type_of(const Tensor& t) {
   switch (t.scalar_type()) {
     case torch::kFloat32: return ATOMO_F32;
@@ -201,7 +209,10 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
       d["splits"] = (int64_t)a.splits;
       d["count"] = a.count != 0;
       d["per_row"] = reduction == kNone;
-      if (fused) d["grad"] = grad;
+      if (fused) {
+        d["grad"] = grad;
+        d["capture"] = capture_of(stream);
+      }
     }
     return loss;
   }
@@ -241,11 +252,13 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
     a.stats = stats.data_ptr<float>();
     a.up = up.data_ptr<float>();
     a.up_per_row = d["per_row"].toBool();
+    const hipStream_t stream = cur_stream();
     // The gradient that the forward pass wrote is given away once; a further
-    // backward pass makes its own.
+    // backward pass makes its own.  So does one that is captured apart from
+    // the forward pass: its graph may be replayed more than once for each.
     Tensor grad;
     const auto found = d.find("grad");
-    if (found != d.end()) {
+    if (found != d.end() && d["capture"].toInt() == capture_of(stream)) {
       grad = found->second.toTensor();
       d.erase(found);
       a.skip_one = 1;
@@ -256,7 +269,7 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
     a.grad_splits =
         atomo_logit_splits(z.size(0), a.classes, a.type, &a.grad_part);
     if (z.size(0) > 0) {
-      atomo_distill_grad_launch(&a, cur_stream());
+      atomo_distill_grad_launch(&a, stream);
       C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     return {grad,     Tensor(), Tensor(), Tensor(), Tensor(),

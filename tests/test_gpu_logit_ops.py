@@ -439,6 +439,43 @@ def test_distill_in_a_graph(rows, classes, dtype):
         assert torch.equal(loss, want_loss) and torch.equal(grad, want)
 
 
+@pytest.mark.parametrize("rows,classes,dtype", [(128, 100, F32), (130, 20000, BF16)])
+def test_distill_backward_in_a_graph_of_its_own(rows, classes, dtype):
+    """The backward pass's graph makes the gradient on each replay, also where
+    its last result was changed and no forward pass came between."""
+    _, first = _logits(rows, classes, dtype)
+    value, index = (t.cuda() for t in _teacher(rows, classes, 8))
+    y = _labels(rows, classes).cuda()
+    kw = dict(temperature=2.0, weight=0.5)
+    static = first.clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad(logit_ops.distill_loss(static, value, index, y, **kw), static)
+    torch.cuda.current_stream().wait_stream(side)
+    one = torch.ones((), device="cuda")
+    ahead, back = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(ahead, stream=side):
+        loss = logit_ops.distill_loss(static, value, index, y, **kw)
+    with torch.cuda.graph(back, pool=ahead.pool(), stream=side):
+        (grad,) = torch.autograd.grad(loss, static, one)
+    for seed in range(3):
+        _, now = _logits(rows, classes, dtype, seed=seed)
+        with torch.no_grad():
+            static.copy_(now)
+        leaf = now.clone().requires_grad_()
+        want = logit_ops.distill_loss(leaf, value, index, y, **kw)
+        (want_grad,) = torch.autograd.grad(want, leaf)
+        ahead.replay()
+        for _ in range(2):
+            back.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(loss.detach(), want.detach())
+            assert torch.equal(grad, want_grad)
+            grad.zero_()
+
+
 def test_teacher_answers_feed_the_loss():
     """The two together, as they are used: a teacher's alternatives, the
     student's loss and gradient."""
