@@ -53,6 +53,38 @@ def test_fuse_takes_over_parameters():
     assert list(before) == list(after) and all(before[n] is after[n] for n in before)
 
 
+def test_fused_linears_of_modules_that_are_shared_hooked_or_their_own():
+    nn = torch.nn
+
+    class Backwards(nn.Sequential):
+        def forward(self, x):
+            for layer in reversed(self):
+                x = layer(x)
+            return x
+
+    torch.manual_seed(0)
+    act, norm = nn.ReLU(), nn.Hardtanh(-4.0, -1.0)
+    shared = nn.Linear(6, 6)
+    hooked = nn.Linear(6, 6)
+    hooked.register_forward_hook(lambda layer, args, out: out + 1)
+    watched = nn.ReLU()
+    watched.register_forward_hook(lambda layer, args, out: out - 1)
+    model = nn.Sequential(
+        nn.Linear(6, 6), norm, nn.Linear(6, 6), norm, act, shared, act, shared,
+        hooked, nn.ReLU(), nn.Linear(6, 6), watched,
+        Backwards(nn.Linear(6, 6), nn.ReLU(), nn.Linear(6, 6)))
+    for p in model.parameters():
+        p.data = torch.randint(-1, 2, p.shape).float()  # whole numbers: exact sums
+    x = torch.randint(-1, 2, (50, 6)).float()
+    want = model(x)
+    keys = list(model.state_dict())
+    got = fuse_linears(model)(x)
+    assert want.abs().max() < 2 ** 20 and torch.equal(got, want)
+    assert list(model.state_dict()) == keys and model[8] is hooked
+    assert [m.activation for m in model if isinstance(m, FusedLinear)] == [
+        "none", "none", "relu", "none", "none"]
+
+
 def test_answers_are_loss_accuracy_and_entropy():
     g = torch.Generator().manual_seed(0)
     z, y = torch.randn(50, 10, generator=g), torch.randint(0, 10, (50,), generator=g)
