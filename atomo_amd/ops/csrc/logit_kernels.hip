@@ -1099,7 +1099,7 @@ __global__ void __launch_bounds__(1024)
   if (threadIdx.x % WAVE == 0) lds[threadIdx.x / WAVE] = n;
   __syncthreads();
   if (threadIdx.x == 0) {
-    int all = 0;
+    int64_t all = 0;
     for (int i = 0; i < 1024 / WAVE; ++i) all += lds[i];
     *inverse = 1.0f / (float)(all > 0 ? all : 1);
   }
