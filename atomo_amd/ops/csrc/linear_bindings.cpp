@@ -149,9 +149,17 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     // What the three steps need in between lies in one piece of memory, in
     // turn: the products' parts and db's block sums.
     const bool make_dp = slope.defined() && (want_x || want_w);
+    Tensor dp = make_dp ? torch::empty({m, n}, x.options()) : dy;
     AtomoProduct px{}, pw{};
     int64_t work = 0;
     if (want_x) {
+      dx = torch::empty({m, k}, x.options());
+      px.p = weight.data_ptr();
+      px.ldp = row_stride(weight);
+      px.q = dp.data_ptr();
+      px.ldq = row_stride(dp);
+      px.out = dx.data_ptr();
+      px.ldo = k;
       px.form = ATOMO_GRAD_X;
       px.type = type;
       px.ni = (int)k;
@@ -161,6 +169,13 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       work = std::max(work, parts_of(px));
     }
     if (want_w) {
+      dw = torch::empty({n, k}, x.options());
+      pw.p = x.data_ptr();
+      pw.ldp = row_stride(x);
+      pw.q = dp.data_ptr();
+      pw.ldq = row_stride(dp);
+      pw.out = dw.data_ptr();
+      pw.ldo = k;
       pw.form = ATOMO_GRAD_W;
       pw.type = type;
       pw.ni = (int)k;
@@ -177,9 +192,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     const Tensor between = floats(work, x);
     float* partial = between.defined() ? between.data_ptr<float>() : nullptr;
 
-    Tensor dp = dy;
     if (make_dp || want_b) {
-      if (make_dp) dp = torch::empty({m, n}, x.options());
       if (want_b) db = torch::empty({n}, x.options());
       d.dy = dy.data_ptr();
       d.ld_dy = row_stride(dy);
@@ -195,24 +208,10 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       C10_HIP_KERNEL_LAUNCH_CHECK();
     }
     if (want_x) {
-      dx = torch::empty({m, k}, x.options());
-      px.p = weight.data_ptr();
-      px.ldp = row_stride(weight);
-      px.q = dp.data_ptr();
-      px.ldq = row_stride(dp);
-      px.out = dx.data_ptr();
-      px.ldo = k;
       px.partial = partial;
       product(px);
     }
     if (want_w) {
-      dw = torch::empty({n, k}, x.options());
-      pw.p = x.data_ptr();
-      pw.ldp = row_stride(x);
-      pw.q = dp.data_ptr();
-      pw.ldq = row_stride(dp);
-      pw.out = dw.data_ptr();
-      pw.ldo = k;
       pw.partial = partial;
       product(pw);
     }

@@ -40,9 +40,10 @@ struct AtomoProduct {
   int64_t ldp, ldq, ldo, ldr, ld_part;
   int ni, nj, nk;
   int type, form, act;
-  // by atomo_product_plan, from type, form, act, the sizes and which of bias,
-  // residual and slope there are; `bare`: the tiles have no epilogue
-  int plan, splits, k_part, bare;
+  // by atomo_product_plan, from type, form, act, p, q, ldp, ldq, the sizes and
+  // which of bias, residual and slope there are; `bare`: the tiles have no
+  // epilogue, `direct`: operands are loaded straight into LDS
+  int plan, splits, k_part, bare, direct;
 };
 
 // dp = dy * slope, where dp is wanted; db, the sums of its columns, likewise.

@@ -732,6 +732,143 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
                 (float*)lds + wave * pass_floats<kFi>());
 }
 
+// Where 16-bit operands are aligned to 16 bytes and hold whole steps
+// (direct_fits), memory is loaded straight into LDS, without registers in
+// between, and an operand that lies across stays so there: the LDS reads
+// transpose, 4 x 16 elements for each 16 lanes.  Nothing of a step is left to a
+// wave but the loads' issue, a step ahead, and the fragments' reads.  The same
+// sums in the same order as by registers.
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <int kRows, int kThreads, bool kAcross>
+struct Direct {
+  static constexpr int kVecs = kRows * kRowChunks / kThreads;
+  // Rows across: a k's row has kRows / 32 pieces of 64 bytes.  Sixteen lanes
+  // read 32 bytes of four k each: neighbouring k have their pieces exchanged so
+  // that these fall on all banks.
+  __device__ static int turn(int k) {
+    return kRows == 64 ? k >> 1 & 1 : k & 3;
+  }
+  __amdgpu_buffer_rsrc_t from;
+  int at[kVecs];  // bytes, of the thread's vectors in step 0
+  int step;       // bytes from one step to the next
+
+  __device__ __forceinline__ Direct(const uint16_t* p, int64_t ld, int rows) {
+    // offsets are below 2^31 (direct_fits) and in the matrix: rows from `rows`
+    // on are read in the place of the last ones, for results that nobody keeps
+    from = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7FFFFFFF, 0x00027000);
+    step = kAcross ? kRowBytes / 2 * (int)ld * 2 : kRowBytes;
+#pragma unroll
+    for (int s = 0; s < kVecs; ++s) {
+      const int id = threadIdx.x + s * kThreads;
+      if constexpr (!kAcross) {
+        const int row = id / kRowChunks;
+        const int c = (id % kRowChunks) ^ ((row ^ (row >> 3)) & 7);  // slot()
+        at[s] = (min(row, rows - 1) * (int)ld + c * 8) * 2;
+      } else {
+        const int k = id / (kRows / 8), c = id % (kRows / 8);
+        const int row = ((c / 4 ^ turn(k)) * 4 + c % 4) * 8;
+        at[s] = (k * (int)ld + min(row, rows - 8)) * 2;
+      }
+    }
+  }
+
+  // a wave's 64 vectors lie one behind the other in LDS
+  __device__ __forceinline__ void load(u32x4* tile, int s) const {
+    u32x4* to = tile + threadIdx.x / 64 * 64;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          from, (lds_void*)(to + v * kThreads), 16, at[v], s * step, 0, 0);
+  }
+
+  // of rows row..row + 31 the eight k of chunk c + lane / 32
+  __device__ static __forceinline__ u32x4 fragment(const u32x4* tile, int row,
+                                                   int c) {
+    const int lane = threadIdx.x % 64;
+    if constexpr (!kAcross) {
+      return tile[slot(row + lane % 32, c + lane / 32)];
+    } else {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      u32x4 out;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = (c + lane / 32) * 8 + h * 4 + lane % 16 / 4;
+        const char* at = (const char*)tile + k * kRows * 2 +
+                         (row / 32 ^ turn(k)) * 64 + lane % 32 / 16 * 32 +
+                         lane % 4 * 8;
+        const u32x2 r = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+        out[2 * h] = r[0];
+        out[2 * h + 1] = r[1];
+      }
+      return out;
+    }
+  }
+};
+
+// 8192 x 4096 x 4096 bf16, forward / dx / dW: 224 / 240 / 229 us, 1.23 / 1.14 /
+// 1.20 PFLOP/s (by registers 285 / 281 / 282).  Matrix instructions need half
+// of that; LDS takes as long for its reads and writes, and the one barrier of
+// a step keeps parts of the two apart.  Two buffers of their own, so that the
+// compiler sees that reads of one need not wait for loads into the other.
+template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
+          int kWj>
+__global__ void __launch_bounds__(kWi* kWj * 64)
+    product_direct_kernel(AtomoProduct a) {
+#if defined(__HIP_DEVICE_COMPILE__)  // LDS pointers are not the host's
+  constexpr int kThreads = kWi * kWj * 64;
+  constexpr int kFi = kI / kWi / 32, kFj = kJ / kWj / 32;
+  __shared__ u32x4 even[(kI + kJ) * kRowChunks];
+  __shared__ u32x4 odd[(kI + kJ) * kRowChunks];
+  static_assert(kWi * kWj / 2 * pass_floats<kFi>() * 4 <= (int)sizeof(even), "LDS");
+  const int wave = threadIdx.x / 64;
+  const Work<E, kAcrossP, kAcrossQ, kI, kJ> work(a);
+  using P = Direct<kI, kThreads, kAcrossP>;
+  using Q = Direct<kJ, kThreads, kAcrossQ>;
+  const P dp(work.p, a.ldp, work.rows_i);
+  const Q dq(work.q, a.ldq, work.rows_j);
+  const int wi = wave % kWi * (kI / kWi), wj = wave / kWi * (kJ / kWj);
+  f32x16 acc[kFi][kFj] = {};
+  const auto load = [&](u32x4* tile, int s) __attribute__((always_inline)) {
+    s += work.begin;
+    s = s < work.steps ? s : s - work.steps;
+    dp.load(tile, s);
+    dq.load(tile + kI * kRowChunks, s);
+    __builtin_amdgcn_sched_barrier(0);  // before the step, not after it
+  };
+  const auto use = [&](const u32x4* tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < kRowChunks; c += 2) {
+      u32x4 fp[kFi], fq[kFj];
+#pragma unroll
+      for (int t = 0; t < kFi; ++t) fp[t] = P::fragment(tile, wi + t * 32, c);
+#pragma unroll
+      for (int t = 0; t < kFj; ++t)
+        fq[t] = Q::fragment(tile + kI * kRowChunks, wj + t * 32, c);
+      multiply<E>(fp, fq, acc);
+    }
+    // the wave's loads into the other buffer have arrived, then everybody's
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+  };
+  load(even, 0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);
+  __syncthreads();
+  int s = 0;
+  for (; s + 1 < work.steps; s += 2) {
+    load(odd, s + 1);
+    use(even);
+    if (s + 2 < work.steps) load(even, s + 2);
+    use(odd);
+  }
+  if (s < work.steps) use(even);
+  write_tile<E>(a, work.part, work.i0 + wi, work.j0 + wj, acc,
+                (float*)(wave % 2 ? odd : even) + wave / 2 * pass_floats<kFi>());
+#endif
+}
+
 // The same for fp32 operands on the bf16 matrix instructions, 16 times as fast
 // as the fp32 ones: with x = a + b + c and y = a' + b' + c' (put_thirds) the
 // six products aa', ab', ba', bb', ac', ca' are xy but for 2^-25 of it, less
@@ -1060,9 +1197,15 @@ void launch_product(const AtomoProduct& a, hipStream_t stream) {
   if constexpr (E::kChunk == 4 && !kTiny)
     hipLaunchKernelGGL((product_thirds_kernel<kAcrossP, kAcrossQ, kI, kJ, kWi, kWj>),
                        grid, block, 0, stream, a);
-  else
+  else if (!kTiny && a.direct) {
+    if constexpr (E::kChunk == 8 && !kTiny)
+      hipLaunchKernelGGL(
+          (product_direct_kernel<E, kAcrossP, kAcrossQ, kI, kJ, kWj, kWi>), grid,
+          block, 0, stream, a);
+  } else {
     hipLaunchKernelGGL((product_kernel<E, kAcrossP, kAcrossQ, kI, kJ, kWi, kWj, kTiny>),
                        grid, block, 0, stream, a);
+  }
 }
 
 template <typename E, int kI, int kJ, int kWi, int kWj, bool kTiny = false>
@@ -1132,7 +1275,8 @@ void linear_dp(const AtomoLinearDp& a, hipStream_t stream) {
 
 // What a step of 128 bytes of the reduction costs a workgroup, in us: alone on
 // its CU, where it waits for its loads, and as its share of a full one; by
-// type (fp32, 16 bits), form and tile (64, 128, 256).  Measured on products of
+// kernel (fp32, 16 bits by registers, straight into LDS), form and tile (64, 128,
+// 256).  Measured on products of
 // 16 to 8192 by 10 to 4096 by 500 to 9216; the choices that follow from it, and
 // what lies next to them:
 //   1024 x 1024 x 1024 bf16 forward: 64, one part 11 us; 128, four parts 20
@@ -1142,13 +1286,16 @@ void linear_dp(const AtomoLinearDp& a, hipStream_t stream) {
 struct Step {
   float alone, shared;
 };
-constexpr Step kStep[2][3][3] = {
+constexpr Step kStep[3][3][3] = {
     {{{0.90f, 0.56f}, {1.95f, 1.50f}, {}},
      {{1.15f, 0.57f}, {1.85f, 1.50f}, {}},
      {{1.40f, 0.83f}, {1.90f, 1.60f}, {}}},
     {{{0.55f, 0.29f}, {0.90f, 0.98f}, {2.40f, 2.40f}},
      {{0.75f, 0.34f}, {0.95f, 1.05f}, {2.35f, 2.35f}},
-     {{0.95f, 0.60f}, {1.00f, 1.10f}, {2.30f, 2.30f}}}};
+     {{0.95f, 0.60f}, {1.00f, 1.10f}, {2.30f, 2.30f}}},
+    {{{0.37f, 0.25f}, {0.90f, 0.52f}, {1.50f, 1.75f}},
+     {{0.37f, 0.25f}, {1.10f, 0.56f}, {1.80f, 1.88f}},
+     {{0.37f, 0.25f}, {1.05f, 0.55f}, {1.70f, 1.79f}}}};
 constexpr float kTileEnd[3] = {0.25f, 1.4f, 6.f};  // a tile's epilogue
 
 float cost_of(const AtomoProduct& a, int tile, int64_t splits, int steps) {
@@ -1156,7 +1303,8 @@ float cost_of(const AtomoProduct& a, int tile, int64_t splits, int steps) {
   const int size = 64 << tile;
   const int64_t tiles =
       (int64_t)((a.ni + size - 1) / size) * ((a.nj + size - 1) / size);
-  const Step& step = kStep[a.type != ATOMO_F32][a.form][tile];
+  const Step& step =
+      kStep[a.type == ATOMO_F32 ? 0 : a.direct ? 2 : 1][a.form][tile];
   const float per_cu = (float)((tiles * splits + kCus - 1) / kCus);
   float each = step.shared * per_cu;
   if (each < step.alone) each = step.alone;
@@ -1165,6 +1313,15 @@ float cost_of(const AtomoProduct& a, int tile, int64_t splits, int steps) {
   // a launch more, and the sums written and read again at 5.5 TB/s
   if (splits > 1) us += 3.5f + (float)a.ni * a.nj * splits * (8 / 5.5e6f);
   return us;
+}
+
+// Whether an operand may be loaded straight into LDS: 16-byte vectors at
+// aligned places, eight rows or eight k at once, whole steps of 64 k, and byte
+// offsets within a workgroup's part below 2^31.
+bool direct_fits(const void* p, int64_t ld, int rows, int nk, bool across) {
+  if ((uintptr_t)p % 16 != 0 || ld % 8 != 0 || nk % 64 != 0) return false;
+  if (across) return rows % 8 == 0 && ld < ((int64_t)1 << 29) / nk;
+  return ld < (int64_t)1 << 21 && nk < 1 << 29;
 }
 
 }  // namespace
@@ -1180,6 +1337,7 @@ float cost_of(const AtomoProduct& a, int tile, int64_t splits, int steps) {
 extern "C" {
 
 void atomo_product_plan(AtomoProduct* a) {
+  a->direct = 0;
   a->splits = 1;
   a->k_part = a->nk;
   a->ld_part = (a->ni + 3) / 4 * 4;
@@ -1197,6 +1355,9 @@ void atomo_product_plan(AtomoProduct* a) {
     a->plan = ATOMO_PLAN_TINY;
     return;
   }
+  a->direct = a->type != ATOMO_F32 &&
+              direct_fits(a->p, a->ldp, a->ni, a->nk, a->form != ATOMO_FORWARD) &&
+              direct_fits(a->q, a->ldq, a->nj, a->nk, a->form == ATOMO_GRAD_W);
   const int step = kRowBytes / (a->type == ATOMO_F32 ? 4 : 2);
   const int steps = (a->nk + step - 1) / step;
   float least = 0.f;

@@ -67,6 +67,33 @@ def test_exact_sizes(m, k, n, dtype):
     _check_exact(m, k, n, dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,k,n", [
+    (64, 64, 64), (192, 128, 8), (8, 64, 320), (448, 192, 72), (72, 64, 128),
+    (320, 1088, 576), (2048, 64, 2048), (1000, 448, 1992), (384, 2112, 328),
+    (8, 4096, 64), (64, 4096, 8)])
+def test_exact_sizes_of_whole_steps(m, k, n, dtype):
+    """Multiples of eight, and of 64 where sums run over them: operands that
+    go straight to LDS, in one step or an odd or even number, in tiles that
+    pass the last row, and, each by one element, just not."""
+    _check_exact(m, k, n, dtype)
+    _check_exact(m, k, n, dtype, "none", True, False)
+    x, w = (torch.zeros(rows, k + 16, dtype=dtype) for rows in (m, n))
+    for left in (8, 3):
+        vx, vw = x[:, left:left + k], w[:, left:left + k]
+        vx.copy_(_grid((m, k), 6, dtype))
+        vw.copy_(_grid((n, k), 7, dtype))
+        cx, cw = x.cuda()[:, left:left + k], w.cuda()[:, left:left + k]
+        dy = _grid((m, n + 8), 8, dtype).cuda()[:, :n]
+        cx, cw = cx.detach().requires_grad_(), cw.detach().requires_grad_()
+        y = linear_ops.linear_act(cx, cw)
+        gx, gw = torch.autograd.grad(y, (cx, cw), dy)
+        dd = dy.cpu().double()
+        assert torch.equal(y.cpu(), (vx.double() @ vw.double().t()).to(dtype))
+        assert torch.equal(gx.cpu(), (dd @ vw.double()).to(dtype))
+        assert torch.equal(gw.cpu(), (dd.t() @ vx.double()).to(dtype))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("activation,residual,bias", [
     ("none", False, False), ("none", True, True), ("relu", True, False)])
