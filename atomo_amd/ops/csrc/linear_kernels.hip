@@ -13,7 +13,8 @@
 // So the inner loop is the same for all: a 16-byte read for each fragment,
 // which one 16-bit matrix instruction consumes (k = 16) or four fp32 ones
 // (k = 2 each; the order of a sum's terms is free, so lane halves take four
-// neighbouring k each).  p gives the rows of the matrix instruction's result:
+// neighbouring k each).  Aligned 16-bit operands go to LDS directly, as they
+// lie, and are transposed as they are read (product_direct_kernel).  p gives the rows of the matrix instruction's result:
 // a lane then holds four neighbouring i of one j, and stores them at once.
 //
 // Sums are fp32; an output is rounded once.
@@ -678,11 +679,10 @@ __device__ __forceinline__ void write_tile(const AtomoProduct& a, int part,
 
 // kI x kJ of the result by kWi x kWj waves; a tile of the reduction is 128
 // bytes of each row, double-buffered in LDS.  8192 x 4096 x 4096 bf16, forward
-// / dx / dW: 314 / 301 / 296 us, 0.88 / 0.91 / 0.93 PFLOP/s, where a library's
-// products take 182 / 255 / 290.  Matrix instructions need 40 % of the time, LDS
-// reads and writes as much, and the barrier of each step keeps part of them
-// apart.  With several parts of the
-// reduction (`splits`) each leaves its fp32 sums for join_parts_kernel.
+// / dx / dW: 258 / 275 / 276 us, 1.07 / 1.0 / 1.0 PFLOP/s.  Matrix instructions
+// need less than half of the time, LDS reads and writes as much, and the barrier
+// of each step keeps part of them apart.  With several parts of the reduction
+// (`splits`) each leaves its fp32 sums for join_parts_kernel.
 template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
           int kWj, bool kTiny>
 __global__ void __launch_bounds__(kWi* kWj * 64)
@@ -808,10 +808,12 @@ struct Direct {
   }
 };
 
-// 8192 x 4096 x 4096 bf16, forward / dx / dW: 224 / 240 / 229 us, 1.23 / 1.14 /
-// 1.20 PFLOP/s (by registers 285 / 281 / 282).  Matrix instructions need half
-// of that; LDS takes as long for its reads and writes, and the one barrier of
-// a step keeps parts of the two apart.  Two buffers of their own, so that the
+// 8192 x 4096 x 4096 bf16, forward / dx / dW: 221 / 234 / 223 us, 1.24 / 1.17 /
+// 1.23 PFLOP/s (by registers 258 / 275 / 276; a library's products take 182 /
+// 255 / 290).  Matrix instructions need half of that; LDS takes as long for its
+// reads and writes, and the one barrier of a step keeps parts of the two apart.
+// Half of the waves a phase behind the others, so that they read while those
+// multiply: 222 / 269 / 260.  Two buffers of their own, so that the
 // compiler sees that reads of one need not wait for loads into the other.
 template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
           int kWj>
@@ -1279,9 +1281,10 @@ void linear_dp(const AtomoLinearDp& a, hipStream_t stream) {
 // 256).  Measured on products of
 // 16 to 8192 by 10 to 4096 by 500 to 9216; the choices that follow from it, and
 // what lies next to them:
-//   1024 x 1024 x 1024 bf16 forward: 64, one part 11 us; 128, four parts 20
-//   2048 x 2048 x 2048 bf16 forward: 128, one part 37 us; two parts 41
-//   512 x 512 x 4096 bf16 forward: 64, four parts 15 us; one part 31
+//   1024 x 1024 x 1024 bf16 forward: 64, one part 8 us; 128, two parts 16
+//   2048 x 2048 x 2048 bf16 forward: 128, one part 30 us; two parts 38
+//   8192 x 4096 x 4096 bf16 forward: 256, one part 221 us; 128 267; 64 421
+//   512 x 512 x 4096 bf16 forward: 64, eight parts 13 us; four 12, two 15
 //   128 x 9216 -> 4096 fp32 forward: 128, 16 parts 63 us; 8 or 32 parts 75
 struct Step {
   float alone, shared;
