@@ -108,18 +108,22 @@ __device__ __forceinline__ void multiply(const u32x4 (&p)[kI],
 }
 
 // Half the complementary error function of -h / sqrt(2), and exp(-h^2 / 2).
-// Beside 16-bit results: Abramowitz and Stegun, Handbook of Mathematical
-// Functions, 7.1.26, whose error, 0.8e-7 here, is far below their rounding and
-// which shares the exponential; a quarter of the instructions.
+// Beside 16-bit results by their quotient, which varies slowly: a polynomial
+// in t = 1 / (1 + 0.36 |h|), fitted so that its largest relative error over
+// h = -13.5..0 is least, 2^-20; the exponential's exponent, rounded twice, adds
+// h^2 2^-24.  So a result is within 2^-17 of itself down to h = -8 and rounded
+// once.  It costs nothing that can be measured against a polynomial that is
+// good in absolute terms only: 8192 x 4096 x 4096 bf16 with gelu, forward and
+// backward, 801 us with either.
 template <bool kShort>
 __device__ __forceinline__ float normal_cdf(float h, float* bell) {
   if constexpr (kShort) {
-    const float x = fabsf(h) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.36f * fabsf(h));
     const float e = __builtin_amdgcn_exp2f(h * h * -0.72134752044448170f);
     const float p =
-        ((((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t -
-          0.284496736f) * t + 0.254829592f) * t * e * 0.5f;
+        ((((((0.047306422f * t - 0.18061617f) * t + 0.18210846f) * t +
+            0.025755247f) * t + 0.14001004f) * t + 0.14171898f) * t +
+         0.14371689f) * t * e;
     *bell = e;
     return h < 0.f ? p : 1.f - p;
   } else {

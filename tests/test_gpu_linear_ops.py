@@ -301,3 +301,24 @@ def test_in_a_graph(m, k, n, dtype):
         torch.cuda.synchronize()
         for a, c in zip(out, want):
             assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("k", [2, 64, 100])
+@pytest.mark.parametrize("rows", [1, 1793])
+def test_gelu_of_16_bits_is_rounded_once(rows, k, dtype):
+    """h = -8..-1 in steps of 2^-8, as the sum of two numbers that the type
+    holds: each result is the rounding of a number 2^-16 next to gelu(h)."""
+    steps = torch.arange(-2048, -255) if rows > 1 else torch.tensor([-1027])
+    h = steps.double() / 256
+    x = torch.zeros(rows, k, dtype=dtype)
+    x[:, 0] = torch.div(steps, 16, rounding_mode="trunc") / 16
+    x[:, 1] = torch.fmod(steps, 16) / 256
+    w = torch.zeros(24, k, dtype=dtype)
+    w[:, :2] = 1
+    y = linear_ops.linear_act(x.cuda(), w.cuda(), None, "gelu").cpu()
+    want = h * 0.5 * torch.erfc(-h / math.sqrt(2))
+    # exponents of at most 47, rounded twice: 47 * 2^-23; a dozen roundings
+    low = (want * (1 + 2.0 ** -16)).to(dtype)[:, None]
+    high = (want * (1 - 2.0 ** -16)).to(dtype)[:, None]
+    assert ((low <= y) & (y <= high)).all()
