@@ -83,10 +83,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     const bool by_output = act == ATOMO_ACT_RELU && !residual.defined();
     Tensor slope;
     if (train && act != ATOMO_ACT_NONE && !by_output)
-      slope = torch::empty({m, n},
-                           x.scalar_type() == torch::kFloat32
-                               ? x.options()
-                               : x.options().dtype(torch::kInt16));
+      slope = torch::empty({m, n}, x.options().dtype(torch::kFloat32));
     if (m > 0) {
       AtomoProduct a{};
       a.p = weight.data_ptr();

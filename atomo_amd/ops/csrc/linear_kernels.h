@@ -35,7 +35,7 @@ struct AtomoProduct {
   void* out;
   const void* bias;      // or null
   const void* residual;  // or null
-  void* slope;           // act'(.), or null: fp32, or 16 bits (see put_slope)
+  void* slope;           // act'(.) in fp32, or null
   float* partial;        // (splits, nj, ld_part), where splits > 1
   int64_t ldp, ldq, ldo, ldr, ld_part;
   int ni, nj, nk;
@@ -47,7 +47,8 @@ struct AtomoProduct {
 };
 
 // dp = dy * slope, where dp is wanted; db, the sums of its columns, likewise.
-// Without a slope dp is dy; with `by_output` the slope is relu's output.
+// Without a slope dp is dy; with `by_output` the slope is relu's output, in the
+// operands' type, otherwise it is fp32.
 struct AtomoLinearDp {
   const void* dy;
   const void* slope;

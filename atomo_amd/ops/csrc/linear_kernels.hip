@@ -48,7 +48,6 @@ struct F32 {
   static constexpr int kChunk = 4;  // elements in 16 bytes
   __device__ static float widen(Raw r) { return __uint_as_float(r); }
   __device__ static Raw narrow(float f) { return __float_as_uint(f); }
-  using Slope = uint32_t;
 };
 struct BF16 {
   using Raw = uint16_t;
@@ -64,7 +63,6 @@ struct BF16 {
         __builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), acc, 0, 0,
         0);
   }
-  using Slope = uint16_t;
 };
 struct F16 {
   using Raw = uint16_t;
@@ -80,7 +78,6 @@ struct F16 {
         __builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), acc, 0, 0,
         0);
   }
-  using Slope = uint16_t;
 };
 
 // acc[i][j] += the products of 16 bytes of p's rows i and q's rows j
@@ -428,24 +425,6 @@ struct Stage {
   }
 };
 
-// The slope of an activation, kept for the backward pass: fp32 beside fp32
-// operands; beside 16-bit ones a fixed point number of 2^-15 steps from -1/4
-// on, exact at 0 and 1 and 2^-16 off at most.  (Slopes lie in -0.13..1.13.  In
-// bf16 itself this rounding would weigh as much as that of dp.)
-__device__ __forceinline__ void put_slope(uint32_t* at, float s) {
-  *at = __float_as_uint(s);
-}
-__device__ __forceinline__ void put_slope(uint16_t* at, float s) {
-  *at = s != s ? 0xFFFFu : (uint16_t)((int)rintf(s * 32768.f) + 8192);
-}
-__device__ __forceinline__ float slope_of(uint32_t r) {
-  return __uint_as_float(r);
-}
-__device__ __forceinline__ float slope_of(uint16_t r) {
-  return r == 0xFFFFu ? __builtin_nanf("")
-                      : (float)((int)r - 8192) * (1.f / 32768.f);
-}
-
 // neighbours in a row, at the alignment of one
 template <typename Raw, int kN>
 struct Some {
@@ -484,20 +463,22 @@ __device__ __forceinline__ void finish(const AtomoProduct& a, int64_t j, int i,
                                        const Four<typename E::Raw>& bias,
                                        const Four<typename E::Raw>& residual) {
   using Raw = typename E::Raw;
-  using Slope = typename E::Slope;
   Four<Raw> y;
-  Four<Slope> s;
+  // fp32, whatever the operands: the slopes of gelu and silu fall to 0 without
+  // an end, and next to their zero they need digits that 16 bits do not have.
+  // (8192 x 4096 bf16: 67 MB more here and in linear_dp_kernel.)
+  Four<float> s;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     float h = sum[e], d;
     if (a.bias) h += E::widen(bias.v[e]);
     h = activate<E::kChunk == 8>(a.act, h, &d);
-    put_slope(&s.v[e], d);
+    s.v[e] = d;
     if (a.residual) h += E::widen(residual.v[e]);
     y.v[e] = E::narrow(h);
   }
   store_some<4>((Raw*)a.out + j * a.ldo + i, a.ni - i, y);
-  if (a.slope) store_some<4>((Slope*)a.slope + j * a.ni + i, a.ni - i, s);
+  if (a.slope) store_some<4>((float*)a.slope + j * a.ni + i, a.ni - i, s);
 }
 
 template <typename E>
@@ -1085,8 +1066,7 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
       float h = sum[n][m], d;
       if (a.bias) h += E::widen(((const Raw*)a.bias)[n0 + n]);
       h = activate<E::kChunk == 8>(a.act, h, &d);
-      if (a.slope)
-        put_slope((typename E::Slope*)a.slope + (int64_t)m * a.ni + n0 + n, d);
+      if (a.slope) ((float*)a.slope)[(int64_t)m * a.ni + n0 + n] = d;
       if (a.residual)
         h += E::widen(((const Raw*)a.residual)[m * a.ldr + n0 + n]);
       ((Raw*)a.out)[m * a.ldo + n0 + n] = E::narrow(h);
@@ -1105,7 +1085,6 @@ template <typename E, int kV>
 __global__ void __launch_bounds__(kDpWaves * 64)
     linear_dp_kernel(AtomoLinearDp a) {
   using Raw = typename E::Raw;
-  using Slope = typename E::Slope;
   __shared__ float lds[kDpWaves][64 * kV];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int c = (blockIdx.x * 64 + lane) * kV;
@@ -1121,7 +1100,7 @@ __global__ void __launch_bounds__(kDpWaves * 64)
   for (int r0 = first + wave; r0 < last; r0 += kDpWaves * kDepth) {
     if (n <= 0) break;
     Some<Raw, kV> v[kDepth], y[kDepth];
-    Some<Slope, kV> s[kDepth];
+    Some<float, kV> s[kDepth];
     const auto load = [&](int n) {
 #pragma unroll
       for (int u = 0; u < kDepth; ++u) {
@@ -1129,7 +1108,7 @@ __global__ void __launch_bounds__(kDpWaves * 64)
         const int64_t at = r * a.columns + c;
         v[u] = load_some<kV>(dy + r * a.ld_dy + c, n);
         if (by_output) y[u] = load_some<kV>((const Raw*)a.slope + at, n);
-        if (by_slope) s[u] = load_some<kV>((const Slope*)a.slope + at, n);
+        if (by_slope) s[u] = load_some<kV>((const float*)a.slope + at, n);
       }
     };
     // apart, so that whole ones are read without a branch in between
@@ -1147,7 +1126,7 @@ __global__ void __launch_bounds__(kDpWaves * 64)
         if (by_output)
           d = E::widen(y[u].v[e]) <= 0.f ? 0.f : d;
         else if (by_slope)
-          d *= slope_of(s[u].v[e]);
+          d *= s[u].v[e];
         v[u].v[e] = E::narrow(d);
         sum[e] += d;
       }

@@ -55,8 +55,8 @@ def linear_act(
 
     Products and sums are fp32 (fp32 operands are multiplied as such), the
     result is rounded once.  The slope of gelu and silu is kept for the
-    backward pass in fp32, or beside 16-bit operands in steps of 2^-15; dy
-    times the slope is rounded to the operands' type before it is multiplied.
+    backward pass in fp32; dy times the slope is rounded to the operands' type
+    before it is multiplied.
     Rows may be strided; other layouts are copied first.  The gradients cannot
     be differentiated again on a GPU.
     """

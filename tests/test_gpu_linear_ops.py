@@ -322,3 +322,46 @@ def test_gelu_of_16_bits_is_rounded_once(rows, k, dtype):
     low = (want * (1 + 2.0 ** -16)).to(dtype)[:, None]
     high = (want * (1 - 2.0 ** -16)).to(dtype)[:, None]
     assert ((low <= y) & (y <= high)).all()
+
+
+def _tail(m, k, n, dtype, centre):
+    """x, w, b >= 0 or whole steps of 2^-5: h = centre + 0..1 or so, exactly."""
+    g = torch.Generator().manual_seed(m + k + n)
+    x = (torch.rand(m, k, generator=g) < min(1.0, 4.0 / k)).to(dtype)
+    w = (torch.randint(1, 5, (n, k), generator=g) / 32.0).to(dtype)
+    return x, w, torch.full((n,), centre).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("activation,centre", [
+    ("gelu", -4.0), ("gelu", -5.0), ("gelu", -6.0), ("silu", -10.0),
+    ("silu", -13.0), ("silu", -15.0)])
+@pytest.mark.parametrize("m,k,n", [(1, 100, 40), (7, 5, 9), (130, 64, 72), (64, 2048, 64), (33, 70, 41)])
+def test_small_slopes_keep_their_digits(m, k, n, activation, centre, dtype):
+    """Units that are saturated throughout: their gradients have the relative
+    error of the type's own roundings."""
+    x, w, b = _tail(m, k, n, dtype, centre)
+    g = torch.Generator().manual_seed(0)
+    # dp within fp16's normal numbers: slopes are above 4e-8 here
+    dy = (torch.randint(1, 4, (m, n), generator=g) * 8192.0).to(dtype)
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    y = linear_ops.linear_act(*leaves, activation)
+    gx, gw, gb = torch.autograd.grad(y, leaves, dy.cuda())
+    h = x.double() @ w.double().t() + b.double()
+    if activation == "gelu":
+        slope = 0.5 * torch.erfc(-h / math.sqrt(2)) + h * torch.exp(-h * h / 2) / math.sqrt(2 * math.pi)
+    else:
+        s = torch.sigmoid(h)
+        slope = s * (1 + h * (1 - s))
+    dp = dy.double() * slope
+    assert (slope < 0).all() and dp.abs().min() > 2.0 ** -14
+    half = torch.finfo(dtype).eps / 2
+    # nothing cancels: all terms have one sign.  The functions: exponents of at
+    # most 27 are rounded twice, 27 * 2^-23; a dozen roundings of 2^-24, and
+    # cdf against h * density, which are one sign apart, at most 1.1 times
+    own = 2.0 ** -17
+    for got, want, rounded, terms in ((gx, dp @ w.double(), half, n), (gw, dp.t() @ x.double(), half, m),
+                                      (gb, dp.sum(0), 0.0, m)):
+        off = rounded + own + (terms + 4) * U
+        tiny = torch.finfo(dtype).smallest_normal * half
+        assert ((got.cpu().double() - want).abs() <= (off + half * (1 + off)) * want.abs() + tiny).all()
