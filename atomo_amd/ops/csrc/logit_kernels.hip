@@ -918,7 +918,9 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   if (a.grad == nullptr) return;
-  if (st.s == 0.f) {
+  // no distribution, or no term at all: a teacher without an entry adds nothing
+  // to the gradient of a NaN, either
+  if (st.s == 0.f || (!hard && q_sum == 0.f)) {
     write_zeros<E, kThreads>(g, 0, a.classes);
     return;
   }
@@ -1070,6 +1072,10 @@ __global__ void __launch_bounds__(kSweep) distill_grad_kernel(Distill a) {
   const float c1 = hard ? (1.f - a.weight) * scale : 0.f;
   const float wrong =
       hard && !(label >= 0 && label < a.classes) ? nan_value() : 0.f;
+  if (!hard && q_sum == 0.f) {  // no term at all, whatever the logits are
+    write_zeros<E, kSweep>(g, first, end);
+    return;
+  }
   const float pt = (a.weight == 0.f ? 0.f : ct * q_sum) / st.t + wrong;
   const float p1 = c1 / st.s;
   for (int c0 = first; c0 < end; c0 += kSweep * kParts * kV) {

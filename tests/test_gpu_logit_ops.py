@@ -487,3 +487,23 @@ def test_teacher_answers_feed_the_loss():
     assert torch.equal(out.top_index.cpu(), cpu.top_index)
     _check_distill(zs, student, out.top_logprob.cpu(), out.top_index.cpu(),
                    _labels(rows, classes), 2.0, 0.8)
+
+
+@pytest.mark.parametrize("rows,classes,dtype", [
+    (4, 50, F32), (4, 20000, F32), (130, 20000, BF16), (4, 3000, F16), (4, 9001, F16)])
+@pytest.mark.parametrize("labelled", [False, True])
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_distill_absent_teacher_of_an_odd_student(rows, classes, dtype, labelled, reduction):
+    """A teacher's row of absent entries adds nothing, to the gradient either,
+    whatever the student's row holds."""
+    z, _ = _logits(rows, classes, dtype)
+    z[0, 3], z[1, classes - 1], z[2] = math.nan, math.inf, math.nan
+    value, index = _teacher(rows, classes, 3)
+    value[:3] = -math.inf
+    y = torch.zeros(rows, dtype=torch.long) if labelled else None
+    _check_distill(z, z.cuda(), value, index, y, 2.0, 1.0, reduction)
+    leaf = z.cuda().requires_grad_()
+    loss = logit_ops.distill_loss(leaf, value.cuda(), index.cuda(), None if y is None else y.cuda(),
+                                  temperature=2.0, reduction="none")
+    (grad,) = torch.autograd.grad(loss, leaf, torch.full((rows,), 0.5, device="cuda"))
+    assert (loss[:3] == 0).all() and (grad[:3] == 0).all() and (grad[3] != 0).any()
