@@ -9,6 +9,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <limits>
 #include <tuple>
 
 #include "logit_kernels.h"
@@ -131,7 +132,7 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
 
     AtomoDistill a{};
     a.labels = labels_of(labels, z);
-    a.weight = (float)weight;
+    share(a, weight);
     // without the teacher's weight its entries are not looked at
     a.k = weight == 0.0 ? 0 : (int)values.size(1);
     a.tau = weight == 0.0 ? 1.f : (float)tau;
@@ -217,6 +218,15 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
     return loss;
   }
 
+  // The shares of teacher and labels, each rounded by itself: 1 minus a rounded
+  // weight would be off by 2^-25, however little is left.  Neither becomes 0.
+  static void share(AtomoDistill& a, double weight) {
+    a.weight = weight > 0.0 ? std::max((float)weight,
+                                       std::numeric_limits<float>::min())
+                            : 0.f;
+    a.rest = (float)(1.0 - weight);
+  }
+
   static void describe(AtomoDistill& a, const Tensor& z, const Tensor& values,
                        const Tensor& index, const Tensor& inverse) {
     a.logits = z.data_ptr();
@@ -239,7 +249,7 @@ struct DistillLoss : public torch::autograd::Function<DistillLoss> {
     const Tensor up = up_list[0].to(torch::kFloat32).contiguous();
     AtomoDistill a{};
     a.labels = labels_of(labels, z);
-    a.weight = (float)d["weight"].toDouble();
+    share(a, d["weight"].toDouble());
     a.k = (int)d["k"].toInt();
     a.tau = (float)d["tau"].toDouble();
     a.inv_tau = 1.f / a.tau;

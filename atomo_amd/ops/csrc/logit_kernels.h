@@ -43,7 +43,8 @@ struct AtomoDistill {
   const float* up;       // the loss's gradient, one or one a row
   void* grad;
   int64_t row_stride, rows, ignore;
-  float tau, inv_tau, weight;
+  float tau, inv_tau;
+  float weight, rest;    // of the teacher (0 only where k is) and of the labels
   float factor;          // then this, unless the kernel is to
   int count;             // count them itself
   int type, classes, k;

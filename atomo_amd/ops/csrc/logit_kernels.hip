@@ -647,7 +647,7 @@ struct Teacher {
       // used with the sums only, long after
       z[h] = column[h] < 0 ? 0.f : E::widen(z_row[column[h]]);
     }
-    hard = a.labels != nullptr && a.weight != 1.f;
+    hard = a.labels != nullptr && a.rest != 0.f;
     y = -1;
     zy = nan_value();
     if (hard && label >= 0 && label < a.classes) {
@@ -719,9 +719,9 @@ struct Teacher {
     }
     kd = wave_sum(kd);
     float row = 0.f;
-    if (a.weight != 0.f)
+    if (a.k != 0)
       row = a.weight * a.tau * a.tau * (sum != sum ? sum : kd);
-    if (hard) row += (1.f - a.weight) * (logf(st.s) - (zy - o));
+    if (hard) row += a.rest * (logf(st.s) - (zy - o));
     return row;
   }
 
@@ -902,9 +902,9 @@ __global__ void __launch_bounds__(kThreads)
   }
   if (a.mode == kSoftOnly) st.s = st.t;  // only whether it is 0 is asked
   const float scale = lds_scale, q_sum = lds_sum;
-  const bool hard = a.labels != nullptr && a.weight != 1.f;
-  const float ct = a.weight == 0.f ? 0.f : a.weight * a.tau * scale;
-  float c1 = hard ? (1.f - a.weight) * scale : 0.f;
+  const bool hard = a.labels != nullptr && a.rest != 0.f;
+  const float ct = a.k == 0 ? 0.f : a.weight * a.tau * scale;
+  float c1 = hard ? a.rest * scale : 0.f;
   const float wrong =
       hard && !(label >= 0 && label < a.classes) ? nan_value() : 0.f;
   if (wave == 0) {
@@ -924,7 +924,7 @@ __global__ void __launch_bounds__(kThreads)
     write_zeros<E, kThreads>(g, 0, a.classes);
     return;
   }
-  const float pt = (a.weight == 0.f ? 0.f : ct * q_sum) / st.t + wrong;
+  const float pt = (a.k == 0 ? 0.f : ct * q_sum) / st.t + wrong;
   const float p1 = c1 / st.s;
 #pragma unroll
   for (int r = 0; r < kLoads; ++r) {
@@ -1067,16 +1067,16 @@ __global__ void __launch_bounds__(kSweep) distill_grad_kernel(Distill a) {
   __syncthreads();
   const float scale = lds_scale, q_sum = lds_sum;
   const float o = origin(st.m);
-  const bool hard = a.labels != nullptr && a.weight != 1.f;
-  const float ct = a.weight == 0.f ? 0.f : a.weight * a.tau * scale;
-  const float c1 = hard ? (1.f - a.weight) * scale : 0.f;
+  const bool hard = a.labels != nullptr && a.rest != 0.f;
+  const float ct = a.k == 0 ? 0.f : a.weight * a.tau * scale;
+  const float c1 = hard ? a.rest * scale : 0.f;
   const float wrong =
       hard && !(label >= 0 && label < a.classes) ? nan_value() : 0.f;
   if (!hard && q_sum == 0.f) {  // no term at all, whatever the logits are
     write_zeros<E, kSweep>(g, first, end);
     return;
   }
-  const float pt = (a.weight == 0.f ? 0.f : ct * q_sum) / st.t + wrong;
+  const float pt = (a.k == 0 ? 0.f : ct * q_sum) / st.t + wrong;
   const float p1 = c1 / st.s;
   for (int c0 = first; c0 < end; c0 += kSweep * kParts * kV) {
     u32x4 v[kParts];

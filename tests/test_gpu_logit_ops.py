@@ -507,3 +507,40 @@ def test_distill_absent_teacher_of_an_odd_student(rows, classes, dtype, labelled
                                   temperature=2.0, reduction="none")
     (grad,) = torch.autograd.grad(loss, leaf, torch.full((rows,), 0.5, device="cuda"))
     assert (loss[:3] == 0).all() and (grad[:3] == 0).all() and (grad[3] != 0).any()
+
+
+@pytest.mark.parametrize("rows,classes,dtype", [(130, 100, F32), (3, 20000, F32)])
+@pytest.mark.parametrize("weight", [1 - 1e-5, 1 - 1e-7, 1 - 1e-9])
+def test_distill_labels_of_little_weight_have_their_share(rows, classes, dtype, weight):
+    """The labels' share is 1 - weight as given, not as fp32 holds the weight:
+    the teacher is absent, so nothing else is there."""
+    z, cuda = _logits(rows, classes, dtype)
+    value, index = _teacher(rows, classes, 2)
+    value[:] = -math.inf
+    y = torch.arange(rows) % classes
+    leaf = cuda.detach().requires_grad_()
+    kw = dict(temperature=2.0, weight=weight, reduction="sum")
+    loss = logit_ops.distill_loss(leaf, value.cuda(), index.cuda(), y.cuda(), **kw)
+    (grad,) = torch.autograd.grad(loss, leaf)
+    log_p = torch.log_softmax(z.double(), 1)
+    hot = torch.zeros_like(log_p).scatter_(1, y[:, None], 1.0)
+    share = 1.0 - weight
+    # fp32 arithmetic relative to its terms, as in _check_distill
+    u = U * (_steps(classes, _spread(z)) + rows / 64 + 64)
+    size = share * ((-log_p * hot).sum(1) + math.log(classes + 1)).sum()
+    assert abs(float(loss.detach()) + float((log_p * hot).sum() * share)) <= 2 * u * size
+    want = share * (log_p.exp() - hot)
+    assert ((grad.cpu().double() - want).abs() <= 2 * u * share * (log_p.exp() + hot)).all()
+    # a wrong label makes the row NaN at any share
+    y[0] = classes
+    loss = logit_ops.distill_loss(leaf, value.cuda(), index.cuda(), y.cuda(), **kw)
+    assert loss.isnan()
+
+
+@pytest.mark.parametrize("classes", [50, 20000])
+def test_distill_teacher_of_next_to_no_weight_is_looked_at(classes):
+    """A weight that fp32 rounds to 0 is not 0: a wrong class makes NaN."""
+    z, cuda = _logits(3, classes, F32)
+    value, index = _teacher(3, classes, 2)
+    index[1, 0] = classes
+    _check_distill(z, cuda, value, index, torch.tensor([1, 2, 3]), 2.0, 1e-50, "none")
