@@ -6,6 +6,8 @@ import threading
 import pytest
 import torch
 
+from side_by_side import run_threads
+
 from atomo_amd.ops.linear_ops import linear_act
 from atomo_amd.ops.logit_ops import distill_loss, label_logprobs
 
@@ -103,3 +105,19 @@ def test_two_graphs_in_turn():
             eager = jobs[1 - i]()
             torch.cuda.synchronize()
             assert _equal(outs[i], want[i]) and _equal(eager, want[1 - i])
+
+
+def test_threads_side_by_side_make_all_of_their_passes():
+    """The same with what a thread raises, and passes that are counted."""
+    jobs = [_job(i) for i in range(3)]
+    want = [run() for run in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            out = jobs[i]()
+            streams[i].synchronize()
+        assert _equal(out, want[i])
+
+    run_threads([lambda i=i: work(i) for i in range(3)], 5)
