@@ -88,9 +88,11 @@ def linear_act(
     if activation == "relu":
         h = h.relu()
     elif activation != "none":
-        # 0 at -inf, their limit
-        h = h.clamp_min(-1e4)
-        h = F.gelu(h) if activation == "gelu" else F.silu(h)
+        # at both ends their limits, with the slopes 0 and 1
+        far = h.detach().abs() > 1e4
+        act = F.gelu if activation == "gelu" else F.silu
+        near = act(h.masked_fill(far, 0.0))
+        h = torch.where(far, h.masked_fill(h.detach() < 0.0, 0.0), near)
     if residual is not None:
         h = h + residual.double()
     return h.to(x.dtype)

@@ -365,3 +365,18 @@ def test_small_slopes_keep_their_digits(m, k, n, activation, centre, dtype):
         off = rounded + own + (terms + 4) * U
         tiny = torch.finfo(dtype).smallest_normal * half
         assert ((got.cpu().double() - want).abs() <= (off + half * (1 + off)) * want.abs() + tiny).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("activation", ["none", "relu", "gelu", "silu"])
+def test_slopes_at_the_ends_are_the_oracles(activation, dtype):
+    x = torch.tensor([[math.inf], [-math.inf], [3e4], [-3e4], [math.nan]], dtype=dtype)
+    w = torch.ones(1, 1, dtype=dtype)
+    for residual in (None, torch.zeros(5, 1, dtype=dtype)):
+        cpu, gpu = x.clone().requires_grad_(), x.cuda().requires_grad_()
+        y = linear_ops.linear_act(cpu, w, None, activation, residual)
+        z = linear_ops.linear_act(gpu, w.cuda(), None, activation,
+                                  None if residual is None else residual.cuda())
+        torch.testing.assert_close(z.cpu(), y, rtol=0, atol=0, equal_nan=True)
+        (a,), (b,) = torch.autograd.grad(y.sum(), cpu), torch.autograd.grad(z.sum(), gpu)
+        torch.testing.assert_close(b.cpu(), a, rtol=0, atol=0, equal_nan=True)

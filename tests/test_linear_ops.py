@@ -125,3 +125,14 @@ def test_layer_under_autocast():
         assert y.dtype == torch.bfloat16
         y.float().sum().backward()
     assert fused.weight.grad.dtype == torch.float32
+
+
+@pytest.mark.parametrize("activation,slopes", [
+    ("none", [1.0, 1.0, 1.0, 1.0, 1.0]), ("relu", [1.0, 0.0, 1.0, 0.0, 1.0]),
+    ("gelu", [1.0, 0.0, 1.0, 0.0, math.nan]), ("silu", [1.0, 0.0, 1.0, 0.0, math.nan])])
+def test_slopes_at_the_ends(activation, slopes):
+    """Infinities have the slope that the activation tends to; NaN passes."""
+    x = torch.tensor([[math.inf], [-math.inf], [3e4], [-3e4], [math.nan]], requires_grad=True)
+    y = linear_act(x, torch.ones(1, 1), None, activation)
+    (grad,) = torch.autograd.grad(y.sum(), x)
+    torch.testing.assert_close(grad[:, 0], torch.tensor(slopes), rtol=0, atol=0, equal_nan=True)
