@@ -21,6 +21,7 @@ from . import ext
 
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_APPLY = {"none": lambda h: h, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}
 
 
 def _same(t: torch.Tensor, x: torch.Tensor, shape, name: str) -> torch.Tensor:
@@ -90,8 +91,7 @@ def linear_act(
     elif activation != "none":
         # at both ends their limits, with the slopes 0 and 1
         far = h.detach().abs() > 1e4
-        act = F.gelu if activation == "gelu" else F.silu
-        near = act(h.masked_fill(far, 0.0))
+        near = _APPLY[activation](h.masked_fill(far, 0.0))
         h = torch.where(far, h.masked_fill(h.detach() < 0.0, 0.0), near)
     if residual is not None:
         h = h + residual.double()
@@ -106,7 +106,8 @@ def linear_relu(layer: nn.Module, x: torch.Tensor) -> torch.Tensor:
 
 class FusedLinear(nn.Linear):
     """``nn.Linear`` with its activation in the same kernel; same parameters,
-    same names."""
+    same names.  Types that the kernel does not take (fp64) go the way of
+    ``nn.Linear``."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True,
                  activation: str = "none"):
@@ -135,6 +136,9 @@ class FusedLinear(nn.Linear):
             x, weight = x.to(kind), weight.to(kind)
             bias = bias if bias is None else bias.to(kind)
             residual = residual if residual is None else residual.to(kind)
+        if x.dtype not in _FLOATS:
+            y = _APPLY[self.activation](F.linear(x, weight, bias))
+            return y if residual is None else y + residual
         return linear_act(x, weight, bias, self.activation, residual)
 
     def extra_repr(self) -> str:

@@ -187,3 +187,10 @@ def test_wrong_distillation_is_refused(tmp_path, wrong):
 def test_many_classes_keep_the_top():
     z = torch.randn(3, 300)
     assert label_logprobs(z, top=128).top_index.shape == (3, 128)
+
+
+def test_fused_models_take_double_precision():
+    plain, fused = (build_model("FC", 10, 1, fused_linear=f).double() for f in (False, True))
+    fused.load_state_dict(plain.state_dict())
+    x = torch.randn(2, 1, 28, 28, dtype=torch.float64)
+    assert torch.equal(fused(x), plain(x))

@@ -136,3 +136,18 @@ def test_slopes_at_the_ends(activation, slopes):
     y = linear_act(x, torch.ones(1, 1), None, activation)
     (grad,) = torch.autograd.grad(y.sum(), x)
     torch.testing.assert_close(grad[:, 0], torch.tensor(slopes), rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("activation", sorted(PLAIN))
+def test_layer_takes_what_a_linear_takes(activation):
+    """fp64, which gradcheck asks for."""
+    torch.manual_seed(0)
+    linear = nn.Linear(6, 4).double()
+    fused = FusedLinear.of(linear, activation)
+    x = torch.randn(3, 6, dtype=torch.float64, requires_grad=True)
+    r = torch.randn(3, 4, dtype=torch.float64)
+    assert torch.equal(fused(x), PLAIN[activation](linear(x)))
+    assert torch.equal(fused(x, r), PLAIN[activation](linear(x)) + r)
+    assert torch.autograd.gradcheck(fused, (x,))
+    with pytest.raises(TypeError):
+        fused(x.float())
