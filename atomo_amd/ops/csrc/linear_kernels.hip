@@ -45,12 +45,14 @@ typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
 
 struct F32 {
   using Raw = uint32_t;
+  static constexpr Raw kMinusZero = 0x80000000u;
   static constexpr int kChunk = 4;  // elements in 16 bytes
   __device__ static float widen(Raw r) { return __uint_as_float(r); }
   __device__ static Raw narrow(float f) { return __float_as_uint(f); }
 };
 struct BF16 {
   using Raw = uint16_t;
+  static constexpr Raw kMinusZero = 0x8000u;
   static constexpr int kChunk = 8;
   __device__ static float widen(Raw r) {
     return __uint_as_float((uint32_t)r << 16);
@@ -66,6 +68,7 @@ struct BF16 {
 };
 struct F16 {
   using Raw = uint16_t;
+  static constexpr Raw kMinusZero = 0x8000u;
   static constexpr int kChunk = 8;
   __device__ static float widen(Raw r) {
     return (float)__builtin_bit_cast(_Float16, r);
@@ -154,6 +157,20 @@ __device__ __forceinline__ float activate(int act, float h, float* slope) {
   }
   *slope = 1.f;
   return h;
+}
+
+// An output from its fp32 value.  Of relu without a residual the backward pass
+// reads the slope off the output: a value above 0 that the type rounds to 0
+// (fp16: below 2^-25) is written as -0, which is equal to 0, and is not lost.
+template <typename E>
+__device__ __forceinline__ typename E::Raw output(const AtomoProduct& a, float y) {
+  const typename E::Raw r = E::narrow(y);
+  const bool lost = a.act == ATOMO_ACT_RELU && !a.residual && y > 0.f && r == 0;
+  return lost ? E::kMinusZero : r;
+}
+template <typename E>
+__device__ __forceinline__ bool relu_is_off(typename E::Raw y) {
+  return E::widen(y) <= 0.f && y != E::kMinusZero;
 }
 
 constexpr int kRowBytes = 128;  // of the reduction, in a tile
@@ -475,7 +492,7 @@ __device__ __forceinline__ void finish(const AtomoProduct& a, int64_t j, int i,
     h = activate<E::kChunk == 8>(a.act, h, &d);
     s.v[e] = d;
     if (a.residual) h += E::widen(residual.v[e]);
-    y.v[e] = E::narrow(h);
+    y.v[e] = output<E>(a, h);
   }
   store_some<4>((Raw*)a.out + j * a.ldo + i, a.ni - i, y);
   if (a.slope) store_some<4>((float*)a.slope + j * a.ni + i, a.ni - i, s);
@@ -1069,7 +1086,7 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
       if (a.slope) ((float*)a.slope)[(int64_t)m * a.ni + n0 + n] = d;
       if (a.residual)
         h += E::widen(((const Raw*)a.residual)[m * a.ldr + n0 + n]);
-      ((Raw*)a.out)[m * a.ldo + n0 + n] = E::narrow(h);
+      ((Raw*)a.out)[m * a.ldo + n0 + n] = output<E>(a, h);
     }
   }
 }
@@ -1124,7 +1141,7 @@ __global__ void __launch_bounds__(kDpWaves * 64)
       for (int e = 0; e < kV; ++e) {
         float d = E::widen(v[u].v[e]);
         if (by_output)
-          d = E::widen(y[u].v[e]) <= 0.f ? 0.f : d;
+          d = relu_is_off<E>(y[u].v[e]) ? 0.f : d;
         else if (by_slope)
           d *= s[u].v[e];
         v[u].v[e] = E::narrow(d);

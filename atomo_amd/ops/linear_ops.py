@@ -58,6 +58,8 @@ def linear_act(
     result is rounded once.  The slope of gelu and silu is kept for the
     backward pass in fp32; dy times the slope is rounded to the operands' type
     before it is multiplied.
+    A result of relu that is above 0 and too small for the type is -0, which
+    keeps its slope of 1.
     Rows may be strided; other layouts are copied first.  The gradients cannot
     be differentiated again on a GPU.
     """

@@ -380,3 +380,25 @@ def test_slopes_at_the_ends_are_the_oracles(activation, dtype):
         torch.testing.assert_close(z.cpu(), y, rtol=0, atol=0, equal_nan=True)
         (a,), (b,) = torch.autograd.grad(y.sum(), cpu), torch.autograd.grad(z.sum(), gpu)
         torch.testing.assert_close(b.cpu(), a, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,k,n", [(1, 40, 9), (3, 5, 7), (70, 100, 40), (130, 64, 72), (64, 2048, 64)])
+def test_relu_of_what_rounds_to_zero_has_its_slope(m, k, n, residual, dtype):
+    """Sums of 2^-26, 0 and -2^-26: below fp16's smallest number, but of a
+    sign."""
+    x = torch.zeros(m, k, dtype=dtype)
+    x[:, 0] = 2.0 ** -13 * (torch.arange(m) % 3 - 1 if m > 1 else 1)
+    w = torch.zeros(n, k, dtype=dtype)
+    w[:, 0] = 2.0 ** -13
+    dy = _grid((m, n), 5, dtype)
+    leaves = [t.cuda().requires_grad_() for t in (x, w)]
+    r = torch.zeros(m, n, dtype=dtype, device="cuda") if residual else None
+    y = linear_ops.linear_act(*leaves, None, "relu", r)
+    gx, gw = torch.autograd.grad(y, leaves, dy.cuda())
+    h = x.double() @ w.double().t()
+    dp = dy.double() * (h > 0)
+    assert torch.equal(y.cpu(), h.relu().to(dtype))
+    assert torch.equal(gx.cpu(), (dp @ w.double()).to(dtype))
+    assert torch.equal(gw.cpu(), (dp.t() @ x.double()).to(dtype))
