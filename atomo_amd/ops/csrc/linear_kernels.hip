@@ -876,7 +876,9 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
 // The same for fp32 operands on the bf16 matrix instructions, 16 times as fast
 // as the fp32 ones: with x = a + b + c and y = a' + b' + c' (put_thirds) the
 // six products aa', ab', ba', bb', ac', ca' are xy but for 2^-25 of it, less
-// than fp32 loses by its sums.  2.7 times less time in matrix
+// than fp32 loses by its sums, as long as the parts are normal numbers: what
+// of an operand lies below 2^-126 may count as 0 (operands from 2^-101 on lose
+// nothing).  2.7 times less time in matrix
 // instructions: 8192 x 4096 x 4096 forward in 1.4 ms, 0.2 PFLOP/s, above the
 // 0.157 of the fp32 ones; 128 x 9216 x 4096, forward / dx / dW, in 63 / 72 / 72
 // us (by fp32 instructions 100 / 109 / 139).  There the weight's 151 MB take

@@ -54,8 +54,10 @@ def linear_act(
     (out, in), bias (out), residual (..., out), all of one type: fp32, bf16 or
     fp16.
 
-    Products and sums are fp32 (fp32 operands are multiplied as such), the
-    result is rounded once.  The slope of gelu and silu is kept for the
+    Sums are fp32, the result is rounded once.  fp32 operands of more than
+    four rows are multiplied as three bf16 parts each, six products of nine:
+    to 2^-25 of a product, but what a part holds below 2^-126 may count as 0,
+    so that operands below 2^-101 have fewer digits.  The slope of gelu and silu is kept for the
     backward pass in fp32; dy times the slope is rounded to the operands' type
     before it is multiplied.
     A result of relu that is above 0 and too small for the type is -0, which

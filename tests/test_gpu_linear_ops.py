@@ -402,3 +402,19 @@ def test_relu_of_what_rounds_to_zero_has_its_slope(m, k, n, residual, dtype):
     assert torch.equal(y.cpu(), h.relu().to(dtype))
     assert torch.equal(gx.cpu(), (dp @ w.double()).to(dtype))
     assert torch.equal(gw.cpu(), (dp.t() @ x.double()).to(dtype))
+
+
+@pytest.mark.parametrize("size", [-101, -112, -120])
+@pytest.mark.parametrize("m,k,n", [(3, 50, 20), (130, 200, 140), (40, 3000, 70)])
+def test_tiny_fp32_operands_are_held_to_2_126(m, k, n, size):
+    """Times numbers of 2^100, so that what is lost shows in normal results."""
+    g = torch.Generator().manual_seed(k)
+    x = torch.randn(m, k, generator=g) * 2.0 ** size
+    w = torch.randn(n, k, generator=g) * 2.0 ** 100
+    y = linear_ops.linear_act(x.cuda(), w.cuda()).cpu().double()
+    want = x.double() @ w.double().t()
+    mass = x.abs().double() @ w.abs().double().t()
+    # an operand's parts, each below 2^-126 (the second and third together
+    # 1 + 2^-8 of it), dropped products and fp32's k sums
+    lost = 2.0 ** -126 * (1 + 2.0 ** -8) * w.abs().double().sum(1)
+    assert ((y - want).abs() <= lost + (k + 4) * U * mass).all()
