@@ -681,9 +681,9 @@ __device__ __forceinline__ void write_tile(const AtomoProduct& a, int part,
 
 // kI x kJ of the result by kWi x kWj waves; a tile of the reduction is 128
 // bytes of each row, double-buffered in LDS.  8192 x 4096 x 4096 bf16, forward
-// / dx / dW: 258 / 275 / 276 us, 1.07 / 1.0 / 1.0 PFLOP/s.  Matrix instructions
-// need less than half of the time, LDS reads and writes as much, and the barrier
-// of each step keeps part of them apart.  With several parts of the reduction
+// / dx / dW, bare products of uniform numbers: 258 / 275 / 276 us, 1.07 / 1.0 /
+// 1.0 PFLOP/s.  Matrix instructions need less than half of the time, LDS reads
+// and writes as much, and the barrier of each step keeps part of them apart.  With several parts of the reduction
 // (`splits`) each leaves its fp32 sums for join_parts_kernel.
 template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
           int kWj, bool kTiny>
@@ -810,13 +810,18 @@ struct Direct {
   }
 };
 
-// 8192 x 4096 x 4096 bf16, forward / dx / dW: 221 / 234 / 223 us, 1.24 / 1.17 /
-// 1.23 PFLOP/s (by registers 258 / 275 / 276; a library's products take 182 /
-// 255 / 290).  Matrix instructions need half of that; LDS takes as long for its
-// reads and writes, and the one barrier of a step keeps parts of the two apart.
+// 8192 x 4096 x 4096 bf16, forward / dx / dW, bare products of uniform numbers:
+// 221 / 234 / 223 us, where by registers they take 258 / 275 / 276.  Of normal
+// numbers, in turn with a library's products: 225 / 248 / 241, the library's 180 /
+// 206 / 242.  (The card's clock gives way to what the numbers cost: of zeros 182 /
+// 213 / 203.)  In a pass of forward and backward with gelu and residual, passes
+// in a row: 293 with epilogue and slope / 264 / 261, 0.94 / 1.04 / 1.05 PFLOP/s.
+// Matrix instructions need half of that; LDS takes as long for its reads and
+// writes, and the one barrier of a step keeps parts of the two apart: this
+// arrangement's bound, not the card's, as the library's forward product shows.
 // Half of the waves a phase behind the others, so that they read while those
-// multiply: 222 / 269 / 260.  Two buffers of their own, so that the
-// compiler sees that reads of one need not wait for loads into the other.
+// multiply: 222 / 269 / 260 of uniform numbers.  Two buffers of their own, so
+// that the compiler sees that reads of one need not wait for loads into the other.
 template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
           int kWj>
 __global__ void __launch_bounds__(kWi* kWj * 64)
@@ -880,10 +885,10 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
 // of an operand lies below 2^-126 may count as 0 (operands from 2^-101 on lose
 // nothing).  2.7 times less time in matrix
 // instructions: 8192 x 4096 x 4096 forward in 1.4 ms, 0.2 PFLOP/s, above the
-// 0.157 of the fp32 ones; 128 x 9216 x 4096, forward / dx / dW, in 63 / 72 / 72
-// us (by fp32 instructions 100 / 109 / 139).  There the weight's 151 MB take
-// 27 us; splitting, LDS and matrix instructions as long each, and the barriers
-// keep them apart.  One buffer in LDS, so that three workgroups share a CU and
+// 0.157 of the fp32 ones; 128 x 9216 x 4096, forward / dx / dW, with the parts
+// joined, in 63 / 76 / 78 us (by fp32 instructions 100 / 109 / 139).  There the
+// weight's 151 MB take 27 us and the six products 39 at 1.5 PFLOP/s; splitting
+// and LDS take as long, and the barriers keep them apart.  One buffer in LDS, so that three workgroups share a CU and
 // fill each other's waits.
 //
 // Where a sum comes out infinite or NaN (0 times a split infinity is NaN, and
@@ -997,8 +1002,8 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(AtomoProduct a) {
   finish<E>(a, j, i, sum, bias, residual);
 }
 
-// Few rows, bound by the memory (1 x 9216 -> 4096 bf16 in 13 us, 5.7 TB/s; in
-// tiles 138 us): the weight is read once, by waves that each
+// Few rows, bound by the memory (1 x 9216 -> 4096 bf16 in 13 us, 5.8 TB/s; in
+// tiles 16 us; fp32 in 22 us, 6.8 TB/s, part of it from the cache): the weight is read once, by waves that each
 // take kN of its rows and all of x's kM; a lane takes every 64th 16 bytes.
 template <typename E, int kM, int kN>
 __global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
@@ -1095,9 +1100,15 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
 
 // dp, and the sums of the columns of a block of rows.  64 lanes take 64 times
 // kV neighbours of a row, the waves every kDpWaves-th row.  Bound by the
-// memory: 8192 x 4096 bf16 in 45 us, 4.5 TB/s.  kV is four, or one where four
-// would leave most CUs without a workgroup: 128 x 4096 fp32 in 6.5 us (by
-// fours 13), 128 x 800 in 5 (9).
+// memory: 8192 x 4096 bf16 with slopes in 63 us, 4.3 TB/s.  kV is four, or one
+// where four would leave most CUs without a workgroup: 128 x 4096 fp32 in 6.5 us
+// (by fours 13), 128 x 800 in 5 (9).
+//
+// dp is rounded to the operands' type, as the products' operand; db is summed
+// before.  Where the slope is 0 or 1 nothing is rounded.  Else, of 8192 x 4096 x
+// 4096 bf16 with gelu, dx and dW are 0.0023 of their norm off 64 bits: 0.0017 by
+// the rounding of the results, as much by that of dp.  To keep dp's lower part
+// as an operand of its own would double both products, 0.5 of 0.86 ms more.
 constexpr int kDpWaves = 16;
 
 template <typename E, int kV>
@@ -1280,9 +1291,8 @@ void linear_dp(const AtomoLinearDp& a, hipStream_t stream) {
 // What a step of 128 bytes of the reduction costs a workgroup, in us: alone on
 // its CU, where it waits for its loads, and as its share of a full one; by
 // kernel (fp32, 16 bits by registers, straight into LDS), form and tile (64, 128,
-// 256).  Measured on products of
-// 16 to 8192 by 10 to 4096 by 500 to 9216; the choices that follow from it, and
-// what lies next to them:
+// 256).  Measured on bare products of uniform numbers, 16 to 8192 by 10 to 4096
+// by 500 to 9216; the choices that follow from it, and what lies next to them:
 //   1024 x 1024 x 1024 bf16 forward: 64, one part 8 us; 128, two parts 16
 //   2048 x 2048 x 2048 bf16 forward: 128, one part 30 us; two parts 38
 //   8192 x 4096 x 4096 bf16 forward: 256, one part 221 us; 128 267; 64 421
@@ -1347,8 +1357,10 @@ void atomo_product_plan(AtomoProduct* a) {
   a->k_part = a->nk;
   a->ld_part = (a->ni + 3) / 4 * 4;
   a->bare = a->act == ATOMO_ACT_NONE && !a->bias && !a->residual && !a->slope;
-  // Beyond, the vector units bound it: 9216 -> 4096 for 2 / 4 rows, bf16 20 /
-  // 32 us, in tiles 21 / 21; fp32 for 4 / 8 rows 49 / 63 us, in tiles 56 / 56.
+  // Beyond, its vector instructions bound it, where tiles grow little with the
+  // rows.  At the border, 2 rows so / 3 in tiles, bf16: 512 -> 512 2.9 / 4.3 us,
+  // 2048 -> 2048 4.5 / 6.3, 4096 -> 4096 8.3 / 9.8, 9216 -> 4096 20 / 16; 4 rows
+  // so / 5 in tiles, fp32: 4.5 / 7.4, 12 / 11, 25 / 23, 49 / 45.
   if (a->form == ATOMO_FORWARD && a->nj <= (a->type == ATOMO_F32 ? 4 : 2)) {
     a->plan = ATOMO_PLAN_FEW_ROWS;
     return;
