@@ -137,9 +137,10 @@ class FusedLinear(nn.Linear):
         weight, bias = self.weight, self.bias
         if torch.is_autocast_enabled(x.device.type):
             kind = torch.get_autocast_dtype(x.device.type)
-            x, weight = x.to(kind), weight.to(kind)
-            bias = bias if bias is None else bias.to(kind)
-            residual = residual if residual is None else residual.to(kind)
+            # as torch's own layers: fp64 stays
+            x, weight, bias, residual = (
+                t if t is None or t.dtype == torch.float64 else t.to(kind)
+                for t in (x, weight, bias, residual))
         if x.dtype not in _FLOATS:
             y = _APPLY[self.activation](F.linear(x, weight, bias))
             return y if residual is None else y + residual

@@ -151,3 +151,11 @@ def test_layer_takes_what_a_linear_takes(activation):
     assert torch.autograd.gradcheck(fused, (x,))
     with pytest.raises(TypeError):
         fused(x.float())
+
+
+def test_double_precision_stays_under_autocast():
+    linear = nn.Linear(6, 4).double()
+    x = torch.randn(3, 6, dtype=torch.float64)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        y = FusedLinear.of(linear)(x)
+        assert y.dtype == torch.float64 and torch.equal(y, linear(x))
