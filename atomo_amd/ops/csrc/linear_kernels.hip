@@ -683,8 +683,9 @@ __device__ __forceinline__ void write_tile(const AtomoProduct& a, int part,
 // bytes of each row, double-buffered in LDS.  8192 x 4096 x 4096 bf16, forward
 // / dx / dW, bare products of uniform numbers: 258 / 275 / 276 us, 1.07 / 1.0 /
 // 1.0 PFLOP/s.  Matrix instructions need less than half of the time, LDS reads
-// and writes as much, and the barrier of each step keeps part of them apart.  With several parts of the reduction
-// (`splits`) each leaves its fp32 sums for join_parts_kernel.
+// and writes as much, and the barrier of each step keeps part of them apart.
+// With several parts of the reduction (`splits`) each leaves its fp32 sums for
+// join_parts_kernel.
 template <typename E, bool kAcrossP, bool kAcrossQ, int kI, int kJ, int kWi,
           int kWj, bool kTiny>
 __global__ void __launch_bounds__(kWi* kWj * 64)
@@ -883,13 +884,13 @@ __global__ void __launch_bounds__(kWi* kWj * 64)
 // six products aa', ab', ba', bb', ac', ca' are xy but for 2^-25 of it, less
 // than fp32 loses by its sums, as long as the parts are normal numbers: what
 // of an operand lies below 2^-126 may count as 0 (operands from 2^-101 on lose
-// nothing).  2.7 times less time in matrix
-// instructions: 8192 x 4096 x 4096 forward in 1.4 ms, 0.2 PFLOP/s, above the
-// 0.157 of the fp32 ones; 128 x 9216 x 4096, forward / dx / dW, with the parts
-// joined, in 63 / 76 / 78 us (by fp32 instructions 100 / 109 / 139).  There the
-// weight's 151 MB take 27 us and the six products 39 at 1.5 PFLOP/s; splitting
-// and LDS take as long, and the barriers keep them apart.  One buffer in LDS, so that three workgroups share a CU and
-// fill each other's waits.
+// nothing).  2.7 times less time in matrix instructions: 8192 x 4096 x 4096
+// forward in 1.4 ms, 0.2 PFLOP/s, above the 0.157 of the fp32 ones; 128 x 9216 x
+// 4096, forward / dx / dW, with the parts joined, in 63 / 76 / 78 us (by fp32
+// instructions 100 / 109 / 139).  There the weight's 151 MB take 27 us and the
+// six products 39 at 1.5 PFLOP/s; splitting and LDS take as long, and the
+// barriers keep them apart.  One buffer in LDS, so that three workgroups share a
+// CU and fill each other's waits.
 //
 // Where a sum comes out infinite or NaN (0 times a split infinity is NaN, and
 // so is what rounds up to one) the tile is made again, by fp32 instructions.
@@ -1003,8 +1004,9 @@ __global__ void __launch_bounds__(kThreads) join_parts_kernel(AtomoProduct a) {
 }
 
 // Few rows, bound by the memory (1 x 9216 -> 4096 bf16 in 13 us, 5.8 TB/s; in
-// tiles 16 us; fp32 in 22 us, 6.8 TB/s, part of it from the cache): the weight is read once, by waves that each
-// take kN of its rows and all of x's kM; a lane takes every 64th 16 bytes.
+// tiles 16 us; fp32 in 22 us, 6.8 TB/s, part of it from the cache): the weight
+// is read once, by waves that each take kN of its rows and all of x's kM; a lane
+// takes every 64th 16 bytes.
 template <typename E, int kM, int kN>
 __global__ void __launch_bounds__(kThreads) few_rows_kernel(AtomoProduct a) {
   using Raw = typename E::Raw;

@@ -57,13 +57,12 @@ def linear_act(
     Sums are fp32, the result is rounded once.  fp32 operands of more than
     four rows are multiplied as three bf16 parts each, six products of nine:
     to 2^-25 of a product, but what a part holds below 2^-126 may count as 0,
-    so that operands below 2^-101 have fewer digits.  The slope of gelu and silu is kept for the
-    backward pass in fp32; dy times the slope is rounded to the operands' type
-    before it is multiplied.
-    A result of relu that is above 0 and too small for the type is -0, which
-    keeps its slope of 1.
-    Rows may be strided; other layouts are copied first.  The gradients cannot
-    be differentiated again on a GPU.
+    so that operands below 2^-101 have fewer digits.  The slope of gelu and
+    silu is kept for the backward pass in fp32; dy times the slope is rounded to
+    the operands' type before it is multiplied.  A result of relu that is above
+    0 and too small for the type is -0, which keeps its slope of 1.  Rows may be
+    strided; other layouts are copied first.  The gradients cannot be
+    differentiated again on a GPU.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(
