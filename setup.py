@@ -2,8 +2,8 @@
 
     python setup.py build_ext --inplace
 
-The .so lands at atomo_amd/ops/_atomo_hip*.so so it travels with the repo
-snapshot onto GPU boxes (it is git-ignored but NOT gpurun-ignored).
+The .so lands at atomo_amd/ops/_atomo_hip*.so, beside its sources; it is
+git-ignored.
 """
 
 import os
